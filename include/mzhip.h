@@ -500,6 +500,80 @@ int mz_replay_targets(void* stream, const mz_replay_config_t* config, const int3
                       float* out_target_rewards, float* out_target_values, float* out_target_policies,
                       double* out_total_value);
 
+/* ---- training operators of networks composed outside the built-in kernels ------------------------------------ *
+ * What a training step on the replay targets consists of besides its products.  The reference leaves these to Keras
+ * (training.py:13-51,157-204).  All calls enqueue on `stream` (which belongs to the current device), allocate nothing,
+ * keep nothing between calls and may be captured into a graph; a workspace belongs to one call at a time.  Pointers to
+ * elements are aligned to one element, no further.  Sums and statistics are held in 32 bits or more. */
+typedef enum mz_dtype { MZ_F32 = 0, MZ_F16 = 1, MZ_BF16 = 2 } mz_dtype;
+typedef enum mz_activation { MZ_ACT_NONE = 0, MZ_ACT_RELU = 1, MZ_ACT_SILU = 2, MZ_ACT_GELU = 3 /* by erf */,
+                             MZ_ACT_TANH = 4 } mz_activation;
+
+/* Group norm of channels-last states: for sample n and group g of C / groups channels, over all positions,
+ *   y = activation((x - mean) / sqrt(variance + eps) * weight + bias + residual),   variance of the population.
+ * x, residual and dy (its gradient) are [batch][positions][channels] of `dtype` with a stride (in elements) for batch
+ * and position each and adjacent channels; strides of 0 repeat.  y, dx, dresidual are dense and may not overlap inputs.
+ * weight, bias: [channels] of `param_dtype` (MZ_F32 or `dtype`), each NULL = 1 and 0; residual NULL = none. */
+typedef struct mz_group_norm {
+    int64_t batch, positions;
+    int32_t channels, groups;
+    int32_t dtype, param_dtype;
+    int32_t activation;
+    int32_t reserved;
+    double eps;
+    int64_t x_strides[2], residual_strides[2], dy_strides[2];
+} mz_group_norm_t;
+/* Bytes of workspace that the forward / backward call takes (0: none), or a negative mz_status. */
+int64_t mz_group_norm_workspace(const mz_group_norm_t* config, int32_t backward);
+/* out_mean, out_rstd: [batch][groups] f32 for the backward call, both or neither NULL. */
+int mz_group_norm_forward(void* stream, const mz_group_norm_t* config, const void* x, const void* residual,
+                          const void* weight, const void* bias, void* out_y, float* out_mean, float* out_rstd,
+                          void* workspace, int64_t workspace_bytes);
+/* Any of the four gradients may be NULL.  out_dweight, out_dbias: [channels] of `param_dtype`, summed in a fixed order. */
+int mz_group_norm_backward(void* stream, const mz_group_norm_t* config, const void* x, const void* residual,
+                           const void* weight, const void* bias, const float* mean, const float* rstd, const void* dy,
+                           void* out_dx, void* out_dresidual, void* out_dweight, void* out_dbias,
+                           void* workspace, int64_t workspace_bytes);
+
+/* Cross entropy of K+1 unrolled steps' logits against rows of a replay-target block (mz_replay_targets), without a
+ * gathered copy of them.  Row (u, b) of logits [unroll][batch][classes] meets targets[position[b] + u][game[b]] of
+ * [target_positions][target_games][classes] f32:
+ *   loss[u][b] = w * sum over t_c != 0 of t_c * (log sum exp(z) - z_c),   dlogits = w * (sum(t) * softmax(z) - t).
+ *   position, game: [batch] of index_bytes (4 or 8), each NULL = 0 and b.  A row outside the block gives NaN.
+ *   weights [unroll][batch] f32 by weight_strides (NULL = 1); a row of weight 0 is not looked at: loss and gradient 0.
+ *   A row whose logits are all -inf (nothing left by a mask) has loss and gradient 0.
+ *   dloss [unroll][batch] f32 by dloss_strides: factor of the gradient alone (NULL = 1).
+ * out_loss [unroll][batch] f32 and out_dlogits (dense, `dtype`): either may be NULL.  classes in [1, 4096]. */
+typedef struct mz_categorical {
+    int64_t unroll, batch;
+    int64_t target_positions, target_games;
+    int32_t classes, dtype;
+    int32_t index_bytes;
+    int32_t reserved;
+    int64_t logits_strides[2], weight_strides[2], dloss_strides[2];
+} mz_categorical_t;
+int mz_categorical_loss(void* stream, const mz_categorical_t* config, const void* logits, const float* targets,
+                        const void* game, const void* position, const float* weights, const float* dloss,
+                        float* out_loss, void* out_dlogits);
+
+/* Global norm of n tensors (HOST array of descriptions), sqrt of the sum of all squares (summed in 64 bits, in a fixed
+ * order), to out_norm (one f32), and clipping by it: out = g * max_norm / norm where norm > max_norm, else g.
+ *   outputs: n data pointers (HOST array), same sizes and types; outputs[i] = tensors[i].data or outputs = NULL: in
+ *   place.  Otherwise no output may overlap another tensor's memory, nor two tensors clipped in place each other's.
+ *   workspace: MZ_GLOBAL_NORM_WORKSPACE bytes of device memory.  n in [1, MZ_GLOBAL_NORM_MAX_TENSORS]. */
+typedef struct mz_tensor {
+    void* data;
+    int64_t elements;
+    int32_t dtype;
+    int32_t reserved;
+} mz_tensor_t;
+#define MZ_GLOBAL_NORM_MAX_TENSORS 8192
+#define MZ_GLOBAL_NORM_WORKSPACE 32768
+int mz_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* workspace, int64_t workspace_bytes,
+                   float* out_norm);
+int mz_clip_by_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* const* outputs, double max_norm,
+                           void* workspace, int64_t workspace_bytes, float* out_norm);
+
 #ifdef __cplusplus
 }
 #endif

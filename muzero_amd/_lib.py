@@ -55,6 +55,30 @@ class ReplayConfig(ctypes.Structure):
                 ('value_min', c_double), ('value_max', c_double), ('reward_min', c_double), ('reward_max', c_double)]
 
 
+class GroupNorm(ctypes.Structure):
+    """mz_group_norm_t"""
+    _fields_ = [('batch', c_int64), ('positions', c_int64), ('channels', c_int32), ('groups', c_int32), ('dtype', c_int32),
+                ('param_dtype', c_int32), ('activation', c_int32), ('reserved', c_int32), ('eps', c_double),
+                ('x_strides', c_int64 * 2), ('residual_strides', c_int64 * 2), ('dy_strides', c_int64 * 2)]
+
+
+class Categorical(ctypes.Structure):
+    """mz_categorical_t"""
+    _fields_ = [('unroll', c_int64), ('batch', c_int64), ('target_positions', c_int64), ('target_games', c_int64),
+                ('classes', c_int32), ('dtype', c_int32), ('index_bytes', c_int32), ('reserved', c_int32),
+                ('logits_strides', c_int64 * 2), ('weight_strides', c_int64 * 2), ('dloss_strides', c_int64 * 2)]
+
+
+class Tensor(ctypes.Structure):
+    """mz_tensor_t"""
+    _fields_ = [('data', c_void_p), ('elements', c_int64), ('dtype', c_int32), ('reserved', c_int32)]
+
+
+MZ_F32, MZ_F16, MZ_BF16 = 0, 1, 2
+MZ_ACT_NONE, MZ_ACT_RELU, MZ_ACT_SILU, MZ_ACT_GELU, MZ_ACT_TANH = 0, 1, 2, 3, 4
+MZ_GLOBAL_NORM_MAX_TENSORS = 8192
+MZ_GLOBAL_NORM_WORKSPACE = 32768
+
 # name -> (restype, argtypes); every symbol include/mzhip.h declares
 PROTOTYPES = {
     'mz_last_error': (ctypes.c_char_p, []),
@@ -125,6 +149,12 @@ PROTOTYPES = {
                                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     'mz_selfplay_step_record': (ctypes.c_int, [c_void_p, ctypes.POINTER(Env), ctypes.POINTER(History)] + [c_void_p] * 6),
     'mz_replay_targets': (ctypes.c_int, [c_void_p, ctypes.POINTER(ReplayConfig)] + [c_void_p] * 12),
+    'mz_group_norm_workspace': (c_int64, [ctypes.POINTER(GroupNorm), c_int32]),
+    'mz_group_norm_forward': (ctypes.c_int, [c_void_p, ctypes.POINTER(GroupNorm)] + [c_void_p] * 8 + [c_int64]),
+    'mz_group_norm_backward': (ctypes.c_int, [c_void_p, ctypes.POINTER(GroupNorm)] + [c_void_p] * 12 + [c_int64]),
+    'mz_categorical_loss': (ctypes.c_int, [c_void_p, ctypes.POINTER(Categorical)] + [c_void_p] * 8),
+    'mz_global_norm': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
+    'mz_clip_by_global_norm': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_double, c_void_p, c_int64, c_void_p]),
     'mz_env_cartpole_step': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                             c_void_p, c_void_p]),
 }

@@ -1,0 +1,52 @@
+// Element types, vector loads and reductions of the training operators (mz_norm.hip, mz_loss.hip, mz_clip.hip).
+#pragma once
+#include "mz_common.h"
+
+namespace mz {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+inline int dtype_size(int dtype) { return dtype == MZ_F32 ? 4 : dtype == MZ_F16 || dtype == MZ_BF16 ? 2 : 0; }
+
+// V elements that are loaded and stored as one access.  Aligned like ONE element: gfx950 takes a 4-, 8- or 16-byte access at
+// any element address, so rows of odd widths and views at odd offsets keep their wide accesses.
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+    T v[V];
+};
+
+template <typename T, int V>
+__device__ inline Vec<T, V> load(const T* p) {
+    return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ inline void store(T* p, const float (&f)[V]) {
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = (T)f[i];       // one rounding to the stored type, to nearest even
+    *reinterpret_cast<Vec<T, V>*>(p) = r;
+}
+
+template <typename T>
+__device__ inline T wave_sum(T v) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+    return v;
+}
+
+// Sum over a workgroup of THREADS in a fixed order; every thread gets it.  `scratch`: THREADS / 64 entries of LDS.
+template <int THREADS, typename T>
+__device__ inline T block_sum(T v, T* scratch) {
+    v = wave_sum(v);
+    if (THREADS == 64) return v;
+    __syncthreads();                                    // the scratch of an earlier sum is read no more
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+    __syncthreads();
+    T s = scratch[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; ++i) s += scratch[i];
+    return s;
+}
+
+}  // namespace mz

@@ -1,0 +1,222 @@
+"""Operators of a training step on the targets of replay.py: the categorical loss with its gradient (csrc/mz_loss.hip), the
+global gradient norm and clipping by it (csrc/mz_clip.hip).  The reference leaves them to Keras (training.py:13-51,157-204);
+the names follow its framework."""
+import ctypes
+import math
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from ._launch import DTYPES, launch, refuse_capture_of_live_leaves, remember_leaves, require_hip, require_tensor
+from .exceptions import MuZeroError
+
+MAX_CLASSES = 4096
+
+
+# ---- categorical loss ----------------------------------------------------------------------------------------------------
+class _LossCall:
+    """The checked arguments of one loss: [unroll, batch] rows with a stride for each."""
+
+    def __init__(self, logits, targets, game, position, weights):
+        require_tensor('logits', logits, DTYPES)
+        device = self.device = logits.device
+        if logits.dim() < 2 or not 1 <= logits.shape[-1] <= MAX_CLASSES:
+            raise MuZeroError(f'logits must be [..., classes] with 1 to {MAX_CLASSES} classes, got {tuple(logits.shape)}')
+        require_tensor('targets', targets, (torch.float32,), device)
+        if targets.requires_grad:
+            raise MuZeroError('the loss is not differentiable with respect to targets')
+        indexed = game is not None or position is not None
+        if indexed:
+            if logits.dim() != 3:
+                raise MuZeroError(f'with game and position, logits must be [unroll, batch, classes], got {tuple(logits.shape)}')
+            if game is None or position is None:
+                raise MuZeroError('game and position: both or neither')
+            if targets.dim() != 3 or targets.shape[-1] != logits.shape[-1]:
+                raise MuZeroError(f'targets must be [positions, games, {logits.shape[-1]}], got {tuple(targets.shape)}')
+            for name, t in (('game', game), ('position', position)):
+                require_tensor(name, t, (torch.int32, torch.int64), device)
+                if t.shape != logits.shape[1:2]:
+                    raise MuZeroError(f'{name} must have shape ({logits.shape[1]},), got {tuple(t.shape)}')
+            if game.dtype != position.dtype:
+                raise MuZeroError(f'game is {game.dtype}, position {position.dtype}: both must be of one type')
+        elif targets.shape != logits.shape:
+            raise MuZeroError(f'targets have shape {tuple(targets.shape)}, logits {tuple(logits.shape)}')
+        self.shape = logits.shape[:-1]
+        if weights is not None:
+            require_tensor('weights', weights, (torch.float32,), device)
+            if weights.requires_grad:
+                raise MuZeroError('the loss is not differentiable with respect to weights')
+            try:
+                weights = weights.expand(self.shape)
+            except RuntimeError:
+                raise MuZeroError(f'weights of shape {tuple(weights.shape)} do not broadcast to {tuple(self.shape)}') from None
+        require_hip(device)
+        cfg = self.cfg = _lib.Categorical()
+        classes = logits.shape[-1]
+        cfg.classes, cfg.dtype = classes, DTYPES[logits.dtype]
+        if len(self.shape) == 2:
+            cfg.unroll, cfg.batch = self.shape
+            if logits.stride(-1) != 1 and classes > 1:
+                logits = logits.contiguous()
+            cfg.logits_strides[0], cfg.logits_strides[1] = logits.stride(0), logits.stride(1)
+        else:
+            logits = logits.contiguous()
+            cfg.unroll, cfg.batch = 1, math.prod(self.shape)
+            cfg.logits_strides[1] = classes
+        if indexed:
+            cfg.target_positions, cfg.target_games, cfg.index_bytes = targets.shape[0], targets.shape[1], game.element_size()
+            game, position = game.contiguous(), position.contiguous()
+        else:
+            cfg.target_positions, cfg.target_games = cfg.unroll, cfg.batch
+        weights = self._rows(weights, cfg.weight_strides) if weights is not None else None
+        self.tensors = logits, targets.contiguous(), game, position, weights
+
+    def _rows(self, t, strides):
+        """A tensor of the rows' shape as (u, b) strides."""
+        if len(self.shape) == 2:
+            strides[0], strides[1] = t.stride()
+            return t
+        t = t.contiguous()
+        strides[0], strides[1] = 0, 1
+        return t
+
+    def run(self, tensors, with_loss, with_grad, dloss=None):
+        ptr = lambda t: None if t is None else t.data_ptr()
+        logits = tensors[0]
+        loss = torch.empty(self.shape, dtype=torch.float32, device=self.device) if with_loss else None
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=self.device) if with_grad else None
+        if dloss is not None:
+            dloss = self._rows(dloss, self.cfg.dloss_strides)
+        launch(self.device, _lib.load().mz_categorical_loss, ctypes.byref(self.cfg), *[ptr(t) for t in tensors], ptr(dloss),
+               ptr(loss), ptr(grad))
+        return loss, grad
+
+
+class _CategoricalLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, call):
+        ctx.call = call
+        ctx.save_for_backward(*call.tensors)
+        loss, _ = call.run(call.tensors, True, False)
+        call.tensors = None              # what the backward pass needs, autograd keeps and frees
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        return ctx.call.run(ctx.saved_tensors, False, True, dloss)[1], None
+
+
+def categorical_loss(logits: torch.Tensor, targets: torch.Tensor, game: Optional[torch.Tensor] = None,
+                     position: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cross entropy of the rows of `logits` [..., classes] (float32, float16, bfloat16; 1 to 4096 classes) against target
+    distributions (float32): weights * sum over classes of -target * log_softmax(logits), float32 of shape [...].
+
+    Without `game` and `position`, targets has the shape of logits.  With them, targets is a block [positions, games,
+    classes] as replay.compute_targets returns it (policies, or values of a support), logits is [unroll, batch, classes], and
+    row (u, b) meets targets[position[b] + u, game[b]]: no gathered copy.  An index outside the block gives NaN (the host
+    does not look at them).  weights broadcast over the rows; rows of weight 0 are not read and give 0 whatever they hold.  A
+    class with target 0 adds nothing, also where its logit is -inf (an illegal move); a row whose logits are all -inf gives 0.
+    A row of zero targets (past the end of a game) gives 0.  Differentiable once with respect to logits alone."""
+    call = _LossCall(logits, targets, game, position, weights)
+    if not torch.is_grad_enabled() or not logits.requires_grad:
+        return call.run(call.tensors, True, False)[0]
+    refuse_capture_of_live_leaves(call.device, (logits,))
+    return remember_leaves(call.device, _CategoricalLoss.apply(logits, call))
+
+
+def categorical_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, game: Optional[torch.Tensor] = None,
+                              position: Optional[torch.Tensor] = None,
+                              weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """-> (categorical_loss(...), the gradient of its sum with respect to logits, of their shape and type), in one launch
+    and outside autograd: for a step whose factors are all in `weights` (importance of the samples, scale of the unrolled
+    steps), which passes the gradient on with logits.backward(grad)."""
+    call = _LossCall(logits.detach() if isinstance(logits, torch.Tensor) else logits, targets, game, position, weights)
+    return call.run(call.tensors, True, True)
+
+
+# ---- global norm and clipping --------------------------------------------------------------------------------------------
+def _dense(t):
+    """Every element of t's memory span once: contiguous in some order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    span = 1
+    for st, size in sorted((st, size) for st, size in zip(t.stride(), t.shape) if size != 1):
+        if st != span:
+            return False
+        span *= size
+    return True
+
+
+class GradientSet:
+    """The gradients of a network whose buffers stay where they are from step to step (zeroed in place, or written by a
+    captured graph), described once: `global_norm()` and `clip_by_global_norm(max_norm)` then cost their launches alone.
+
+    tensors: float32, float16 and bfloat16 tensors of one device, each dense in some order of its dimensions.  out: the
+    tensors that clipping writes, of the same shapes, strides and types; None = the tensors themselves.  The set keeps the
+    tensors alive.  Results are ordered on the current stream; nothing is kept between calls."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None) -> None:
+        self.tensors: List[torch.Tensor] = list(tensors)
+        self.out = None if out is None else list(out)
+        n = len(self.tensors)
+        if not 1 <= n <= _lib.MZ_GLOBAL_NORM_MAX_TENSORS:
+            raise MuZeroError(f'1 to {_lib.MZ_GLOBAL_NORM_MAX_TENSORS} tensors, got {n}')
+        first = self.tensors[0]
+        self.device = require_tensor('tensor 0', first, DTYPES).device
+        self._table = (_lib.Tensor * n)()
+        for i, t in enumerate(self.tensors):
+            if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES or t.device != self.device:
+                require_tensor(f'tensor {i}', t, DTYPES, self.device)
+            if not _dense(t):
+                raise MuZeroError(f'tensor {i} is not dense: shape {tuple(t.shape)}, strides {t.stride()}')
+            e = self._table[i]
+            e.data, e.elements, e.dtype = t.data_ptr(), t.numel(), DTYPES[t.dtype]
+        self._outputs = None
+        if self.out is not None:
+            if len(self.out) != n:
+                raise MuZeroError(f'{n} tensors, {len(self.out)} outputs')
+            for i, (t, o) in enumerate(zip(self.tensors, self.out)):
+                if not isinstance(o, torch.Tensor) or o.dtype != t.dtype or o.device != t.device or o.shape != t.shape \
+                        or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous())):
+                    raise MuZeroError(f'output {i} must be like its tensor: {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}')
+            self._outputs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in self.out])
+        require_hip(self.device)
+        self._lib = _lib.load()
+
+    def _buffers(self):
+        return (torch.empty(_lib.MZ_GLOBAL_NORM_WORKSPACE, dtype=torch.uint8, device=self.device),
+                torch.empty((), dtype=torch.float32, device=self.device))
+
+    def global_norm(self) -> torch.Tensor:
+        """sqrt of the sum of the squares of all elements of all tensors: a float32 scalar on the device."""
+        ws, norm = self._buffers()
+        launch(self.device, self._lib.mz_global_norm, len(self.tensors), self._table, ws.data_ptr(), ws.numel(), norm.data_ptr())
+        return norm
+
+    def clip_by_global_norm(self, max_norm: float) -> torch.Tensor:
+        """Writes every tensor times max_norm / global norm to its output where the norm is above max_norm, else unchanged,
+        and returns the norm before clipping.  Where that is NaN every output is NaN; where it is infinite, finite elements
+        become 0 and infinite ones NaN."""
+        if not max_norm >= 0:
+            raise MuZeroError(f'max_norm must be >= 0, got {max_norm}')
+        written = self.tensors if self.out is None else self.out
+        if any(t.requires_grad for t in written):
+            raise MuZeroError('a tensor that requires grad cannot be written by clipping')
+        ws, norm = self._buffers()
+        launch(self.device, self._lib.mz_clip_by_global_norm, len(self.tensors), self._table, self._outputs, max_norm,
+               ws.data_ptr(), ws.numel(), norm.data_ptr())
+        torch.autograd.graph.increment_version(written)
+        return norm
+
+
+def global_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
+    """GradientSet(tensors).global_norm(), for tensors that are others in every step."""
+    return GradientSet(tensors).global_norm()
+
+
+def clip_by_global_norm(tensors: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """GradientSet(tensors, out).clip_by_global_norm(max_norm): in place, or into `out`; returns the norm before clipping.
+    Tensors that are written may not share memory with others of the list."""
+    return GradientSet(tensors, out).clip_by_global_norm(max_norm)

@@ -1,0 +1,258 @@
+"""muzero_amd.layers.group_norm (csrc/mz_norm.hip) against oracle/train_oracle.py in 64 bits.  A result is held to the
+oracle's bound on 32-bit rounding plus half a step of its own type."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import train_oracle as to
+
+pytestmark = pytest.mark.gpu
+
+HALF = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.float16, torch.bfloat16)}
+TINY = {t: torch.finfo(t).smallest_normal for t in HALF}       # below it a type's steps no longer shrink
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+# batch, positions, channels, groups, type, activation, residual, parameters (None, 'f32', 'same')
+CASES = [
+    (1, (3, 3), 128, 32, F32, 'relu', False, 'f32'), (5, (2,), 128, 16, F32, 'relu', True, 'f32'),
+    (33, (3, 3), 128, 32, BF16, 'relu', True, 'f32'), (3, (19, 19), 64, 4, BF16, 'silu', True, 'f32'),
+    (2, (19, 19), 256, 16, F16, 'relu', True, 'same'), (2, (7, 5), 146, 73, F32, 'gelu', False, 'f32'),
+    (7, (5, 5), 146, 2, BF16, 'gelu', True, 'f32'), (4, (), 24, 3, F32, 'tanh', False, 'f32'),
+    (9, (), 512, 1, F16, 'silu', True, None), (3, (1,), 8, 8, F32, None, False, 'f32'),
+    (3, (1,), 8, 8, BF16, 'tanh', True, 'f32'), (2, (33, 31), 34, 34, F16, 'gelu', False, 'same'),
+    (2, (5,), 2500, 1, F32, 'relu', True, 'f32'), (2, (3,), 4100, 2, BF16, None, False, 'f32'),
+    (1, (64, 64), 48, 3, F16, 'silu', False, 'f32'), (2, (96, 96), 64, 8, BF16, 'relu', True, 'f32'),
+    (300, (3, 3), 16, 4, F32, 'tanh', True, 'f32'), (4097, (2,), 32, 8, BF16, 'relu', False, 'f32'),
+    (17, (11,), 1, 1, F32, 'gelu', True, 'f32'), (1, (1000,), 3, 3, F32, 'silu', False, None),
+    (6, (9,), 12, 4, F16, 'none32', False, 'f32'), (2, (48, 48), 96, 32, F32, 'relu', True, 'f32'),
+    (13, (6, 6), 320, 20, BF16, 'gelu', False, 'same'), (40, (81,), 80, 5, F16, 'relu', True, 'f32'),
+    (2, (101,), 520, 40, F32, None, True, 'f32'), (3, (37,), 1030, 103, BF16, 'silu', False, 'f32'),
+]
+
+
+def make(case, seed=0):
+    N, shape, C, G, dtype, activation, residual, params = case
+    activation = None if activation == 'none32' else activation
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    noise = lambda *s: torch.randn(*s, generator=gen, device='cuda')
+    x = (noise(N, *shape, C) * (1 + 0.5 * noise(C).abs()) + noise(C)).to(dtype)
+    kind = {None: None, 'f32': torch.float32, 'same': dtype}[params]
+    w, b = (None, None) if kind is None else ((1 + 0.2 * noise(C)).to(kind), (0.2 * noise(C)).to(kind))
+    res = noise(N, *shape, C).to(dtype) if residual else None
+    return x, G, w, b, activation, res, noise(N, *shape, C).to(dtype)
+
+
+def f64(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def rows(t):
+    return None if t is None else f64(t).reshape(t.shape[0], -1, t.shape[-1])
+
+
+def oracle(x, G, w, b, activation, res, eps=1e-5):
+    return to.GroupNormOracle(rows(x), G, f64(w), f64(b), eps, activation, rows(res))
+
+
+def check(name, got, want, off, dtype):
+    got, want, off = f64(got).ravel(), np.ravel(want), np.ravel(off)
+    bound = off + HALF[dtype] * np.abs(want) + TINY[dtype] + HALF[dtype] * off
+    worst = np.abs(got - want) - bound
+    assert not np.isnan(got).any(), name
+    assert (worst <= 0).all(), f'{name}: {np.abs(got - want)[worst.argmax()]:.3g} off at {worst.argmax()}, bound {bound[worst.argmax()]:.3g}'
+
+
+def run_and_check(x, G, w, b, activation, res, dy):
+    from muzero_amd.layers import group_norm
+    o = oracle(x, G, w, b, activation, res)
+    if activation == 'relu':                     # no gradient at the kink: rounding decides the slope there
+        dy = dy.clone()
+        dy.reshape(o.z.shape)[torch.from_numpy(np.abs(o.z) < 1e-3).cuda()] = 0
+    check('y without grad', group_norm(x, G, w, b, activation=activation, residual=res), o.y, o.off_y, x.dtype)
+    leaves = [None if t is None else t.detach().requires_grad_() for t in (x, w, b, res)]
+    y = group_norm(leaves[0], G, leaves[1], leaves[2], activation=activation, residual=leaves[3])
+    assert y.dtype == x.dtype and y.shape == x.shape and y.is_contiguous()
+    check('y', y, o.y, o.off_y, x.dtype)
+    live = [t for t in leaves if t is not None]
+    grads = iter(torch.autograd.grad(y, live, dy))
+    want, off = o.backward(rows(dy))
+    for name, leaf in zip(('dx', 'dweight', 'dbias', 'dresidual'), leaves):
+        if leaf is not None:
+            g = next(grads)
+            assert g.dtype == leaf.dtype and g.shape == leaf.shape
+            check(name, g, want[name], off[name], leaf.dtype)
+
+
+@pytest.mark.parametrize('case', CASES, ids=lambda c: '-'.join(str(v).replace('torch.', '').replace(' ', '') for v in c))
+def test_forward_and_backward_against_the_oracle(case):
+    run_and_check(*make(case))
+
+
+def test_layouts_other_than_dense():
+    x, G, w, b, activation, res, dy = make((6, (5, 7), 48, 4, BF16, 'silu', True, 'f32'), 3)
+    wide = torch.zeros(6, 5, 7, 48 + 18, dtype=BF16, device='cuda')
+    wide[..., 3:51] = x
+    nchw = res.permute(0, 3, 1, 2).contiguous(memory_format=torch.channels_last)
+    cropped = torch.zeros(6, 6, 9, 48, dtype=BF16, device='cuda')
+    cropped[:, :5, :7] = x
+    every_other = torch.zeros(12, 5, 7, 48, dtype=BF16, device='cuda')
+    every_other[::2] = x
+    one = torch.randn(1, 1, 1, 48, device='cuda').to(BF16)
+    for a, r in ((wide[..., 3:51], nchw.permute(0, 2, 3, 1)), (cropped[:, :5, :7], res), (every_other[::2], res), (x, one.expand(6, 5, 7, 48)),
+                 (x.permute(0, 2, 1, 3), res.permute(0, 2, 1, 3)), (x.permute(0, 3, 2, 1).contiguous().permute(0, 3, 2, 1), res)):
+        run_and_check(a, G, w, b, activation, r, dy.reshape(a.shape))
+    # a gradient that repeats one value: sum().backward()
+    leaf = x.detach().requires_grad_()
+    from muzero_amd.layers import group_norm
+    y = group_norm(leaf, G, w, b, activation=activation)
+    (g,) = torch.autograd.grad(y.sum(), leaf)
+    want, off = oracle(x, G, w, b, activation, None).backward(np.ones((6, 35, 48)))
+    check('dx of a sum', g, want['dx'], off['dx'], BF16)
+    # a broadcast residual gets the sum of its gradients, as of any broadcast input
+    r = one.clone().requires_grad_()
+    y = group_norm(x, G, w, b, activation=activation, residual=r.expand(6, 5, 7, 48))
+    (g,) = torch.autograd.grad(y, r, dy)
+    want, _ = oracle(x, G, w, b, activation, one.expand(6, 5, 7, 48)).backward(rows(dy))
+    total = want['dresidual'].sum((0, 1))
+    assert np.abs(f64(g).ravel() - total).max() <= np.abs(want['dresidual']).sum((0, 1)).max() * 2 * HALF[BF16] + 1e-3
+
+
+def test_only_the_gradients_asked_for_and_a_second_backward():
+    from muzero_amd.layers import group_norm
+    x, G, w, b, activation, res, dy = make((4, (9,), 32, 8, F32, 'gelu', True, 'f32'))
+    full = [t.clone().requires_grad_() for t in (x, w, b, res)]
+    y = group_norm(full[0], G, full[1], full[2], activation=activation, residual=full[3])
+    want = torch.autograd.grad(y, full, dy, retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(y, full, dy)))
+    for i in range(4):
+        part = [t.clone().requires_grad_(k == i) for k, t in enumerate((x, w, b, res))]
+        y = group_norm(part[0], G, part[1], part[2], activation=activation, residual=part[3])
+        assert torch.equal(torch.autograd.grad(y, part[i], dy)[0], want[i])
+    with pytest.raises(RuntimeError):                  # differentiable once
+        x2 = x.clone().requires_grad_()
+        (g,) = torch.autograd.grad(group_norm(x2, G, w, b).square().sum(), x2, create_graph=True)
+        torch.autograd.grad(g.sum(), x2)
+
+
+def test_empty_states():
+    from muzero_amd.layers import group_norm
+    for shape in ((0, 3, 8), (2, 0, 8), (0, 8)):
+        x, w = torch.zeros(shape, device='cuda', requires_grad=True), torch.ones(8, device='cuda', requires_grad=True)
+        y = group_norm(x, 2, w, activation='relu')
+        assert y.shape == shape
+        gx, gw = torch.autograd.grad(y, [x, w], torch.zeros(shape, device='cuda'))
+        assert gx.shape == shape and (gw == 0).all()
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+def test_a_value_that_is_not_finite_stays_in_its_group(bad):
+    from muzero_amd.layers import group_norm
+    x, G, w, b, _, _, dy = make((4, (9,), 32, 8, F32, None, False, 'f32'))
+    x[2, 5, 13] = bad                                   # sample 2, group 3
+    leaf = x.requires_grad_()
+    y = group_norm(leaf, G, w, b, activation='silu')
+    (g,) = torch.autograd.grad(y, leaf, dy)
+    hit = torch.zeros(4, 9, 32, dtype=torch.bool, device='cuda')
+    hit[2, :, 12:16] = True
+    for t in (y, g):
+        assert torch.isnan(t[hit]).all() and torch.isfinite(t[~hit]).all()
+
+
+def test_constant_groups_and_large_offsets():
+    from muzero_amd.layers import group_norm
+    x = torch.full((2, 9, 8), 3.0, device='cuda')
+    assert (group_norm(x, 2, bias=torch.arange(8., device='cuda')) == torch.arange(8., device='cuda')).all()
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    x = 1000 + torch.randn(3, 400, 16, generator=gen, device='cuda')           # mean 1000 deviations from 0
+    o = oracle(x, 4, None, None, None, None)
+    check('offset', group_norm(x, 4), o.y, o.off_y, F32)
+
+
+def test_results_do_not_depend_on_the_rest_of_the_batch_or_the_run():
+    from muzero_amd.layers import group_norm
+    x, G, w, b, activation, res, dy = make((64, (9,), 128, 32, BF16, 'relu', True, 'f32'))
+    grads = []
+    for _ in range(3):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, res)]
+        y = group_norm(leaves[0], G, leaves[1], leaves[2], activation=activation, residual=leaves[3])
+        grads.append([y.detach()] + list(torch.autograd.grad(y, leaves, dy)))
+    for other in grads[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(grads[0], other))
+
+
+def test_on_another_stream_and_inside_inference_mode():
+    from muzero_amd.layers import group_norm
+    x, G, w, b, activation, res, _ = make((64, (19, 19), 64, 8, BF16, 'relu', True, 'f32'))
+    want = group_norm(x, G, w, b, activation=activation, residual=res)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.inference_mode():
+        again = group_norm(x, G, w, b, activation=activation, residual=res)
+    side.synchronize()
+    assert torch.equal(want, again)
+
+
+def test_more_than_2_to_the_31_elements():
+    from muzero_amd.layers import group_norm
+    N, S, C = 70000, 961, 32                                                    # 2.15e9 elements
+    x = torch.zeros(N, S, C, dtype=F16, device='cuda')
+    x[0], x[-1] = torch.randn(S, C, device='cuda').to(F16), torch.randn(S, C, device='cuda').to(F16)
+    y = group_norm(x, 4, bias=torch.full((C,), 0.5, device='cuda'))
+    for n in (0, N - 1):
+        o = oracle(x[n:n + 1], 4, None, torch.full((C,), 0.5), None, None)
+        check(f'sample {n}', y[n:n + 1], o.y, o.off_y, F16)
+    assert (y[1:-1] == 0.5).all()
+
+
+@pytest.mark.parametrize('shape', [(16, (3, 3), 128), (2, (64, 64), 48)])
+def test_captured_training_pass_replays_like_the_eager_one(shape):
+    from muzero_amd.layers import group_norm
+    N, spatial, C = shape
+    x, G, w, b, activation, res, dy = make((N, spatial, C, 16, BF16, 'silu', True, 'f32'))
+    leaves = [t.detach().requires_grad_() for t in (x, w, b, res)]
+
+    def step():
+        y = group_norm(leaves[0], G, leaves[1], leaves[2], activation=activation, residual=leaves[3])
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(4):
+        with torch.no_grad():
+            leaves[0].add_(0.25 * (k - 1))
+            dy.mul_(1.5)
+        eager = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(captured, eager)), k
+
+
+def test_capture_beside_a_living_eager_graph_is_refused():
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.layers import group_norm
+    x, w = torch.randn(2, 9, 16, device='cuda'), torch.ones(16, device='cuda', requires_grad=True)
+    alive = group_norm(x, 4, w)
+    with pytest.raises(MuZeroError, match='alive'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            group_norm(x, 4, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):          # nothing to differentiate: nothing to refuse
+        y = group_norm(x, 4, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = group_norm(x, 4, w)
+        (g,) = torch.autograd.grad(y, w, x)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, off = oracle(x, 4, w, None, None, None).backward(rows(x))
+    check('dweight', g, want['dweight'], off['dweight'], F32)

@@ -1,0 +1,425 @@
+"""muzero_amd.training (csrc/mz_loss.hip, csrc/mz_clip.hip) against oracle/train_oracle.py in 64 bits, and a training step
+of a composed network on the replay targets with all of the training operators."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import train_oracle as to
+
+pytestmark = pytest.mark.gpu
+
+HALF = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.float16, torch.bfloat16)}
+TINY = {t: torch.finfo(t).smallest_normal for t in HALF}
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def f64(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def check(name, got, want, off, dtype):
+    got, want, off = f64(got).ravel(), np.ravel(want), np.ravel(off)
+    bound = off + HALF[dtype] * np.abs(want) + TINY[dtype] + HALF[dtype] * off
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid='ignore'):
+        worst = np.where(same, -1.0, np.abs(got - want) - bound)
+    assert (worst <= 0).all(), f'{name}: {got[worst.argmax()]:.9g}, expected {want[worst.argmax()]:.9g} within {bound[worst.argmax()]:.3g}'
+
+
+# ---- categorical loss ----------------------------------------------------------------------------------------------------
+def block(positions, games, classes, seed=0, zero=0.2):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    t = torch.rand(positions, games, classes, generator=gen, device='cuda') ** 4
+    t /= t.sum(-1, keepdim=True)
+    return t * (torch.rand(positions, games, 1, generator=gen, device='cuda') >= zero)
+
+
+def run_and_check(logits, targets, rows, weights, **kw):
+    """rows: the target rows in 64 bits, [..., C]."""
+    from muzero_amd.training import categorical_loss, categorical_loss_and_grad
+    C = logits.shape[-1]
+    z, t = f64(logits).reshape(-1, C), rows.reshape(-1, C)
+    w = None if weights is None else f64(weights.expand(logits.shape[:-1])).ravel()
+    want, dz = to.categorical(z, t, w)
+    off, off_dz = to.categorical_bounds(z, t, w)
+    loss, grad = categorical_loss_and_grad(logits, targets, weights=weights, **kw)
+    assert loss.dtype == F32 and loss.shape == logits.shape[:-1] and grad.dtype == logits.dtype and grad.shape == logits.shape
+    check('loss', loss, want, off, F32)
+    check('gradient', grad, dz, off_dz, logits.dtype)
+    leaf = logits.detach().requires_grad_()
+    loss = categorical_loss(leaf, targets, weights=weights, **kw)
+    check('differentiable loss', loss, want, off, F32)
+    up = torch.linspace(-1, 2, loss.numel(), device='cuda').reshape(loss.shape)
+    (g,) = torch.autograd.grad(loss, leaf, up)
+    _, dz = to.categorical(z, t, w, f64(up).ravel())
+    check('gradient by autograd', g, dz, to.categorical_bounds(z, t, w, f64(up).ravel())[1], logits.dtype)
+    check('loss without grad', categorical_loss(logits, targets, weights=weights, **kw), want, off, F32)
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize('classes', [1, 2, 3, 9, 16, 18, 31, 64, 65, 101, 128, 257, 362, 601, 1000, 1024, 1025, 2047, 4095, 4096])
+def test_loss_against_the_oracle(classes, dtype):
+    rows = 5 if classes > 600 else 37
+    gen = torch.Generator(device='cuda').manual_seed(classes)
+    z = (3 * torch.randn(rows, classes, generator=gen, device='cuda')).to(dtype)
+    t = block(rows, 1, classes, classes)[:, 0]
+    run_and_check(z, t, f64(t), torch.rand(rows, generator=gen, device='cuda') + 0.1)
+
+
+@pytest.mark.parametrize('index', [torch.int32, torch.int64], ids=str)
+@pytest.mark.parametrize('unroll,batch,classes,dtype', [(1, 1, 2, F32), (3, 17, 101, F32), (6, 33, 362, BF16), (6, 5, 601, F16), (2, 300, 9, BF16)])
+def test_loss_against_rows_of_a_target_block(unroll, batch, classes, dtype, index):
+    gen = torch.Generator(device='cuda').manual_seed(batch)
+    P, G = 7 + unroll, 11
+    targets = block(P, G, classes, 3)
+    z = (2 * torch.randn(unroll, batch, classes, generator=gen, device='cuda')).to(dtype)
+    game = torch.randint(0, G, (batch,), generator=gen, device='cuda', dtype=index)
+    position = torch.randint(0, 8, (batch,), generator=gen, device='cuda', dtype=index)
+    game[0], position[0] = G - 1, 7                                   # the block's last rows; the same game and position twice
+    game[-1], position[-1] = game[0].clone(), position[0].clone()
+    rows = f64(targets)[(f64(position).astype(int) + np.arange(unroll)[:, None]), f64(game).astype(int)]
+    for weights in (None, torch.rand(batch, generator=gen, device='cuda'), torch.rand(unroll, 1, generator=gen, device='cuda'),
+                    torch.rand(unroll, batch, generator=gen, device='cuda'), torch.rand(batch, unroll, generator=gen, device='cuda').t(),
+                    torch.tensor(0.5, device='cuda')):
+        run_and_check(z, targets, rows, weights, game=game, position=position)
+    # views: heads side by side in one product's output, indexes and targets with strides
+    heads = torch.zeros(batch, unroll, classes + 5, dtype=dtype, device='cuda').transpose(0, 1)
+    heads[..., 3:3 + classes] = z
+    pairs = torch.stack([game, position], 1)
+    run_and_check(heads[..., 3:3 + classes], targets.transpose(0, 1).contiguous().transpose(0, 1), rows, None, game=pairs[:, 0], position=pairs[:, 1])
+
+
+def test_index_outside_the_block_gives_nan_and_nothing_else():
+    from muzero_amd.training import categorical_loss_and_grad
+    U, C, P, G = 3, 9, 6, 4
+    targets = block(P, G, C, 1, zero=0)
+    position = torch.tensor([0, 3, 4, -1, 0, 0, 2 ** 40, -2 ** 40, 2 ** 63 - 2], device='cuda')
+    game = torch.tensor([0, 3, 0, 0, 4, -1, 0, 0, 0], device='cuda')
+    z = torch.randn(U, 9, C, device='cuda')
+    bad = torch.zeros(U, 9, dtype=torch.bool, device='cuda')
+    bad[2, 2] = True                                                  # positions 4, 5 are inside, 6 is not
+    bad[0, 3] = True                                                  # -1, then 0 and 1: a position below 0 spoils its sample's steps
+    bad[1:, 3] = True
+    bad[:, 4:] = True
+    loss, grad = categorical_loss_and_grad(z, targets, game=game, position=position)
+    assert torch.equal(torch.isnan(loss), bad) and torch.equal(torch.isnan(grad), bad[..., None].expand(U, 9, C))
+    weights = torch.where(bad, 0.0, 1.0)                              # weight 0: not looked at
+    loss, grad = categorical_loss_and_grad(z, targets, game=game, position=position, weights=weights)
+    assert (loss[bad] == 0).all() and (grad[bad] == 0).all() and torch.isfinite(loss).all() and (loss[~bad] > 0).all()
+
+
+@pytest.mark.parametrize('classes', [9, 101, 362, 4096])
+def test_masked_logits_and_values_that_are_not_finite(classes):
+    inf, nan = math.inf, math.nan
+    z = torch.randn(10, classes, device='cuda')
+    t = block(10, 1, classes, 2, zero=0)[:, 0].clone()
+    z[0, 1:] = -inf
+    t[0, 1:] = 0                                    # one legal move
+    z[1] = -inf                                     # none: an empty row
+    z[2, ::2] = -inf                                # a target on an illegal move: infinite loss
+    z[3, 4] = nan
+    z[4, 4] = inf
+    z[5] = torch.finfo(F32).min                     # a mask by the lowest value that leaves nothing: a uniform row
+    z[6, 1:] = torch.finfo(F32).min
+    t[6, 1:] = 0
+    t[7] = 0                                        # zero target row
+    z[8], t[8] = nan, 0
+    z[9] += 1e4
+    w = torch.ones(10, device='cuda')
+    w[8] = 0                                        # NaN in a row of weight 0
+    run_and_check(z, t, f64(t), w)
+    z = z.clamp(min=-6e4)                           # the same by the lowest values of 16 bits
+    run_and_check(torch.where(z < -5e4, torch.tensor(torch.finfo(F16).min, device='cuda'), z.clamp(max=6e4)).half(), t, f64(t), w)
+
+
+def test_loss_shapes_and_empty_batches():
+    from muzero_amd.training import categorical_loss, categorical_loss_and_grad
+    z, t = torch.randn(2, 3, 4, 5, device='cuda'), block(24, 1, 5)[:, 0].reshape(2, 3, 4, 5)
+    run_and_check(z, t, f64(t), torch.rand(3, 1, device='cuda'))
+    run_and_check(z.permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0), t, f64(t), torch.rand(2, 3, 4, device='cuda').permute(0, 1, 2))
+    z, t = z[0], t[0]
+    run_and_check(z.transpose(0, 1), t.transpose(0, 1), f64(t.transpose(0, 1)), None)
+    none = torch.zeros(0, dtype=torch.int32, device='cuda')
+    loss, grad = categorical_loss_and_grad(torch.zeros(3, 0, 5, device='cuda'), block(4, 2, 5), game=none, position=none)
+    assert loss.shape == (3, 0) and grad.shape == (3, 0, 5)
+    leaf = torch.zeros(0, 5, device='cuda', requires_grad=True)
+    assert torch.autograd.grad(categorical_loss(leaf, torch.zeros(0, 5, device='cuda')).sum(), leaf)[0].shape == (0, 5)
+    zero = torch.zeros(2, dtype=torch.int32, device='cuda')
+    loss, _ = categorical_loss_and_grad(torch.zeros(1, 2, 5, device='cuda'), torch.zeros(0, 0, 5, device='cuda'), game=zero, position=zero)
+    assert torch.isnan(loss).all()
+
+
+def test_target_block_of_more_than_2_to_the_31_elements():
+    P, G, C = 60, 9000, 4096                                           # 2.2e9 elements
+    targets = torch.zeros(P, G, C, device='cuda')
+    targets[-1, -1], targets[-2, -1] = block(1, 2, C, 5, zero=0)[0]
+    z = torch.randn(2, 1, C, device='cuda')
+    at = lambda v: torch.tensor([v], device='cuda')
+    run_and_check(z, targets, f64(targets[-2:, -1])[:, None], None, game=at(G - 1), position=at(P - 2))
+
+
+def test_changed_logits_are_noticed_and_the_capture_rule_holds():
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.training import categorical_loss
+    z, t = torch.randn(4, 9, device='cuda', requires_grad=True), block(4, 1, 9)[:, 0]
+    mid = z * 1
+    loss = categorical_loss(mid, t).sum()
+    mid.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    alive = categorical_loss(z, t)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(MuZeroError, match='alive'):
+        with torch.cuda.graph(graph):
+            categorical_loss(z, t)
+    del alive
+
+
+def test_captured_loss_replays_like_the_eager_one():
+    from muzero_amd.training import categorical_loss, categorical_loss_and_grad
+    U, B, C = 4, 33, 101
+    z, targets = torch.randn(U, B, C, device='cuda'), block(12, 7, C, 3)
+    leaf = z.requires_grad_()
+    game, position = torch.randint(0, 7, (B,), device='cuda'), torch.randint(0, 9, (B,), device='cuda')
+
+    def step():
+        loss = categorical_loss(leaf, targets, game, position)
+        (g,) = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+        return [loss.detach(), g, *categorical_loss_and_grad(leaf, targets, game, position)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(4):
+        with torch.no_grad():
+            leaf.mul_(1.25)
+            position.copy_((position + k) % 9)
+        eager = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(captured, eager)), k
+
+
+# ---- global norm and clipping --------------------------------------------------------------------------------------------
+def tensors_of(sizes, dtypes, seed=0, scale=1.0):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    return [(scale * torch.randn(n, generator=gen, device='cuda')).to(dtypes[i % len(dtypes)]) for i, n in enumerate(sizes)]
+
+
+def check_clip(tensors, max_norm, got, norm):
+    """The norm: sums in 64 bits, rounded once to float32.  An output: the scale rounded once, the product once in float32 and
+    once to its type."""
+    want, scale = to.clip([f64(t) for t in tensors], max_norm)
+    assert norm.dtype == F32 and norm.shape == ()
+    assert abs(float(norm) - want) <= want * 1.01 * to.U32
+    for i, (t, g) in enumerate(zip(tensors, got)):
+        assert g.dtype == t.dtype and g.shape == t.shape
+        check(f'tensor {i}', g, f64(t) * scale, np.abs(f64(t)) * scale * 2 * to.U32, t.dtype)
+
+
+SIZES = [[1], [0, 5, 0], [3, 1, 2, 7, 8, 9], [16384], [16383, 16385, 1], [100003, 4, 65536], [5] * 127, [5] * 128, [33] * 129, [1000] * 300]
+
+
+@pytest.mark.parametrize('sizes', SIZES, ids=lambda s: f'{len(s)}x{s[0]}')
+@pytest.mark.parametrize('dtypes', [(F32,), (BF16,), (F32, BF16, F16)], ids=['f32', 'bf16', 'mixed'])
+def test_clip_against_the_oracle(sizes, dtypes):
+    from muzero_amd.training import GradientSet, clip_by_global_norm, global_norm
+    tensors = tensors_of(sizes, dtypes)
+    true = to.clip([f64(t) for t in tensors], 1.0)[0]
+    assert abs(float(global_norm(tensors)) - true) <= true * 1.01 * to.U32
+    for max_norm in (0.1, 0.0, 1e6, math.inf):
+        out = [torch.full_like(t, 7) for t in tensors]
+        before = [t.clone() for t in tensors]
+        norm = clip_by_global_norm(tensors, max_norm, out=out)
+        check_clip(tensors, max_norm, out, norm)
+        assert all(torch.equal(a, b) for a, b in zip(tensors, before))
+        inplace = [t.clone() for t in tensors]
+        grads = GradientSet(inplace)
+        norm2 = grads.clip_by_global_norm(max_norm)
+        assert torch.equal(norm, norm2) and all(torch.equal(a, b) for a, b in zip(inplace, out))
+        assert torch.equal(grads.global_norm(), global_norm(inplace))
+
+
+def test_clip_of_views_at_odd_addresses_into_one_flat_buffer():
+    from muzero_amd.training import GradientSet
+    for dtype in (F32, F16, BF16):
+        flat_in = torch.randn(40001, device='cuda').to(dtype)
+        flat_out = torch.full((40002,), 5.0, device='cuda', dtype=dtype)
+        cuts = [1, 2, 130, 131, 9000, 33333, 40001]
+        src = [flat_in[a:b] for a, b in zip(cuts, cuts[1:])]
+        dst = [flat_out[a + 1:b + 1] for a, b in zip(cuts, cuts[1:])]
+        norm = GradientSet(src, dst).clip_by_global_norm(0.5)
+        check_clip(src, 0.5, dst, norm)
+        assert (flat_out[:2] == 5).all()
+        norm = GradientSet(src).clip_by_global_norm(0.5)                 # neighbours in one buffer, in place
+        assert all(torch.equal(a, b) for a, b in zip(src, dst))
+
+
+def test_clip_of_tensors_dense_in_another_order():
+    from muzero_amd.training import GradientSet, clip_by_global_norm
+    a = torch.randn(4, 6, 5, 3, device='cuda').contiguous(memory_format=torch.channels_last)
+    b = torch.randn(7, 9, device='cuda').t()
+    c = torch.randn(1, 5, 1, device='cuda').expand(1, 5, 1)
+    out = [torch.empty_like(t) for t in (a, b, c)]
+    assert out[0].stride() == a.stride() and out[1].stride() == b.stride()
+    check_clip([a, b, c], 0.3, out, clip_by_global_norm([a, b, c], 0.3, out=out))
+    copies = [t.clone() for t in (a, b, c)]
+    versions = [t._version for t in copies]
+    GradientSet(copies).clip_by_global_norm(0.3)
+    assert all(torch.equal(p, q) for p, q in zip(copies, out)) and all(t._version > v for t, v in zip(copies, versions))
+
+
+def test_clip_partly_in_place_and_refusals_on_the_device():
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.training import GradientSet, clip_by_global_norm
+    a, b = torch.randn(100, device='cuda'), torch.randn(50, device='cuda')
+    want = clip_by_global_norm([a, b], 0.5, out=(ref := [torch.empty_like(a), torch.empty_like(b)]))
+    mixed = [a.clone(), torch.empty_like(b)]
+    assert torch.equal(clip_by_global_norm([mixed[0], b], 0.5, out=mixed), want)
+    assert all(torch.equal(p, q) for p, q in zip(mixed, ref))
+    for tensors, out in (([a, a], None), ([a, a[10:]], None), ([a, b], [b.new_empty(100), a[:50]]), ([a[:50], b], [b, a[:50]])):
+        with pytest.raises(MuZeroError, match='overlap'):
+            clip_by_global_norm(tensors, 0.5, out=out)
+    with pytest.raises(MuZeroError, match='requires grad'):
+        clip_by_global_norm([a.clone().requires_grad_()], 0.5)
+    with pytest.raises(MuZeroError):
+        clip_by_global_norm([a], -1.0)
+    with pytest.raises(MuZeroError):
+        clip_by_global_norm([a, b.cpu()], 1.0)
+    twice = GradientSet([a, a]).global_norm()                            # reading the same tensor twice is fine
+    assert abs(float(twice) - math.sqrt(2) * float(GradientSet([a]).global_norm())) <= 3e-7 * float(twice)
+
+
+def test_norms_out_of_the_range_of_32_bit_squares_and_not_finite():
+    from muzero_amd.training import clip_by_global_norm, global_norm
+    for size in (1e30, 1e-30):
+        t = [torch.full((1000,), size, device='cuda'), torch.full((24,), size, device='cuda')]
+        assert abs(float(global_norm(t)) - 32 * size) <= 32 * size * 2 * to.U32
+        clip_by_global_norm(t, size)
+        assert torch.allclose(t[0], torch.full((1000,), size / 32, device='cuda'), rtol=3 * to.U32, atol=0)
+    for bad, others in ((math.nan, math.nan), (math.inf, 0.0)):
+        t = [torch.ones(100, device='cuda'), torch.ones(100, device='cuda', dtype=BF16)]
+        t[0][3] = bad
+        norm = clip_by_global_norm(t, 1.0)
+        assert math.isnan(float(norm)) if math.isnan(bad) else math.isinf(float(norm))
+        assert torch.isnan(t[0][3]) and torch.equal(torch.isnan(t[1]), torch.full((100,), math.isnan(others), device='cuda'))
+        assert others != 0.0 or (t[1] == 0).all()
+
+
+def test_clip_of_more_than_2_to_the_31_elements():
+    from muzero_amd.training import GradientSet
+    n = 2 ** 31 + 12345
+    t = torch.zeros(n, dtype=BF16, device='cuda')
+    t[-3:] = torch.tensor([3.0, 4.0, 12.0])
+    t[0] = 84.0
+    s = GradientSet([t])
+    assert float(s.global_norm()) == 85.0
+    s.clip_by_global_norm(8.5)
+    assert torch.equal(t[-3:].float().cpu(), torch.tensor([0.3, 0.4, 1.2]).to(BF16).float()) and t[0] == torch.tensor(8.4).to(BF16)
+    assert t[1:-3].count_nonzero() == 0
+
+
+def test_captured_clipping_replays_like_the_eager_one():
+    from muzero_amd.training import GradientSet
+    tensors = tensors_of([5, 70000, 333], (F32, BF16))
+    start = [t.clone() for t in tensors]
+    grads = GradientSet(tensors)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = grads.clip_by_global_norm(1.0)
+    for k in range(4):
+        for t, s in zip(tensors, start):
+            t.copy_(s * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = [(s * (k + 1)).clone() for s in start]
+        want = GradientSet(eager).clip_by_global_norm(1.0)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, want) and all(torch.equal(a, b) for a, b in zip(tensors, eager)), k
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------
+def test_a_training_step_on_replay_targets():
+    """Games -> compute_targets -> a residual network on 3x3 boards unrolled twice -> losses against the target block ->
+    gradients -> clipping; every gradient against the same step in 64 bits."""
+    from muzero_amd.layers import group_norm
+    from muzero_amd.replay import compute_targets
+    from muzero_amd.training import categorical_loss, clip_by_global_norm
+    from test_replay_gpu import history_from, make_config
+    rng = np.random.default_rng(3)
+    M, games, A, K, support, B, C = 9, 12, 9, 2, 30, 24, 32
+    lengths = rng.integers(5, M + 1, games)
+    policies = rng.dirichlet(np.ones(A), (M, games)).astype(np.float32)
+    history = history_from(dict(policies=policies, actions=rng.integers(0, A, (M, games)), rewards=rng.random((M, games)),
+                                root_values=rng.random((M, games)) * 5, lengths=lengths))
+    config = make_config(A, 1, 0.997, K, 3, support, (0.0, 40.0))
+    targets = compute_targets(history, config)
+    game = torch.from_numpy(rng.integers(0, games, B)).cuda()
+    position = torch.from_numpy(rng.integers(0, 5, B)).cuda()
+    importance = torch.from_numpy(rng.random(B).astype(np.float32) + 0.5).cuda()
+    scale = importance * torch.tensor([1.0, 0.5, 0.5], device='cuda')[:, None]
+    gen = torch.Generator().manual_seed(1)
+    make = lambda *s: torch.randn(*s, generator=gen) / math.sqrt(s[0])
+    shapes = dict(stem=(27, 9 * C), mix1=(C, C), w1=(C,), b1=(C,), mix2=(C, C), w2=(C,), b2=(C,), act=(A, C), policy=(9 * C, A), value=(9 * C, support + 1))
+    start = {k: (make(*s) if len(s) > 1 else torch.full(s, 1.0 if k[0] == 'w' else 0.1)) for k, s in shapes.items()}
+    board = torch.randn(B, 27, generator=gen)
+
+    def unrolled(p, obs, norm):
+        """-> policy and value logits [K+1, B, .]"""
+        actions = targets['extended_actions'].to(obs.device)
+        h = (obs @ p['stem']).reshape(B, 9, C)
+        out = []
+        for k in range(K + 1):
+            if k:
+                h = h + p['act'][actions[position.to(obs.device) + k - 1, game.to(obs.device)].long()][:, None]
+            r = norm(h @ p['mix1'], p['w1'], p['b1'], None)
+            h = norm(r @ p['mix2'], p['w2'], p['b2'], h)
+            flat = h.reshape(B, -1)
+            out.append((flat @ p['policy'], flat @ p['value']))
+        return [torch.stack(o) for o in zip(*out)]
+
+    params = {k: v.cuda().requires_grad_() for k, v in start.items()}
+    norm = lambda x, w, b, res: group_norm(x, 4, w, b, activation='silu', residual=res)
+    logits, values = unrolled(params, board.cuda(), norm)
+    loss = categorical_loss(logits, targets['target_policies'], game, position, scale) + \
+        0.25 * categorical_loss(values, targets['target_values'], game, position, scale)
+    loss.sum().backward()
+
+    exact = {k: v.double().requires_grad_() for k, v in start.items()}
+
+    def norm64(x, w, b, res):
+        g = x.reshape(B, 9, 4, C // 4)
+        d = g - g.mean((1, 3), keepdim=True)
+        z = (d / torch.sqrt((d * d).mean((1, 3), keepdim=True) + 1e-5)).reshape(B, 9, C) * w + b + (0 if res is None else res)
+        return z * torch.sigmoid(z)
+
+    logits64, values64 = unrolled(exact, board.double(), norm64)
+    steps = torch.arange(K + 1)[:, None]
+
+    def cross_entropy(z, block_):
+        t = block_.cpu().double()[position.cpu() + steps, game.cpu()]
+        return -(t * torch.log_softmax(z, -1)).sum(-1) * scale.cpu().double()
+    want = cross_entropy(logits64, targets['target_policies']) + 0.25 * cross_entropy(values64, targets['target_values'])
+    want.sum().backward()
+    # a chain of about thirty 32-bit operations: each gradient tensor within 1e-4 of its own size in the 2-norm (float32's
+    # half step 6e-8, times the chain, times the factor by which the norms and the unrolled products may enlarge an error)
+    np.testing.assert_allclose(f64(loss), f64(want), rtol=1e-4, atol=1e-4)
+    for k in params:
+        g, e = f64(params[k].grad), f64(exact[k].grad)
+        assert np.linalg.norm(g - e) <= 1e-4 * np.linalg.norm(e), k
+    grads = [p.grad for p in params.values()]
+    flat = torch.zeros(sum(g.numel() for g in grads), device='cuda')
+    out, at = [], 0
+    for g in grads:
+        out.append(flat[at:at + g.numel()].view(g.shape))
+        at += g.numel()
+    total = clip_by_global_norm(grads, 0.5, out=out)
+    check_clip(grads, 0.5, out, total)
+    assert abs(float(torch.linalg.vector_norm(flat.double())) - 0.5) < 1e-6
