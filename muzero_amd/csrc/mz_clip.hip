@@ -47,7 +47,7 @@ __device__ double squares(const T* p, long n) {
     for (long i = threadIdx.x; i < whole; i += kThreads) {
         const Vec<T, V> v = mz::load<T, V>(p + i * V);
 #pragma unroll
-        for (int k = 0; k < V; ++k) s = fma((double)(float)v.v[k], (double)(float)v.v[k], s);
+        for (int k = 0; k < V; ++k) s = fma((double)v[k], (double)v[k], s);
     }
     for (long i = whole * V + threadIdx.x; i < n; i += kThreads) s = fma((double)(float)p[i], (double)(float)p[i], s);
     return s;
@@ -87,7 +87,7 @@ __device__ void scale_chunk(const T* in, T* out, long n, float f) {
         const Vec<T, V> v = mz::load<T, V>(in + i * V);
         float r[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) r[k] = (float)v.v[k] * f;
+        for (int k = 0; k < V; ++k) r[k] = v[k] * f;
         mz::store<T, V>(out + i * V, r);
     }
     for (long i = whole * V + threadIdx.x; i < n; i += kThreads) out[i] = (T)((float)in[i] * f);

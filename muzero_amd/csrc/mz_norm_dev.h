@@ -1,0 +1,716 @@
+// Device code of group norm with residual and activation over channels-last states, forward and backward (include/mzhip.h).
+//
+// Per sample n and group g of D = C / G channels, M = positions * D values:
+//   mu = sum x / M, v = sum (x - mu)^2 / M, r = 1 / sqrt(v + eps), h = (x - mu) r, z = h w_c + b_c + residual, y = act(z)
+//   dz = dy act'(z), db_c = sum dz, dw_c = sum dz h, a = sum_group dz w / M, q = sum_group dz w h / M,
+//   dx = r (dz w - a - q h), dresidual = dz
+// Bound by memory: forward reads x (and residual) and writes y, backward reads x, dy (and residual) and writes dx (and
+// dresidual); 10 to 40 operations a value.
+//
+// A workgroup takes a tile of a sample: whole groups side by side, at least a 128-byte line of channels where there are as
+// many.  A thread keeps one vector of V channels (V divides D: one group a vector) and walks down the positions, so
+// consecutive lanes read consecutive addresses.  Vectors of a group and groups of a tile are padded to powers of two over
+// the lanes: a lane's group, vector and position come from bits of its number, and a group's sum is a butterfly over the
+// other bits (group_sum), without index tables or divisions.  Two ways through:
+//   resident  the tile's values stay in registers between the statistics and the result: one launch, every input read once.
+//   split     samples too large for that (K vectors a thread do not hold the tile): positions are cut into chunks over
+//             several workgroups; a first launch leaves each chunk's partial sums, a second adds them up and reads again.
+// The variance is a sum of squared deviations from the mean (resident) or from the partial means, merged (split): no
+// difference of large sums.  Every sum has one order, so results repeat bit for bit.
+#pragma once
+#include "mz_vec.h"
+#include <cmath>
+#include <type_traits>
+
+namespace mz_norm {
+
+using mz::Vec;
+
+constexpr int kSplitThreads = 256;
+constexpr int kMostSplits = 64;
+
+struct Norm {
+    long N, S;
+    int C, G, D, act, params_f32;
+    float eps;
+    long xs[2], rs[2], ds[2];
+    // lanes: bits [vector in group : ldv][group in tile : lgs][position : lrows][sample : the rest]
+    int ldv, lgs, lrows, samples;
+    int gs, tiles, pieces;                    // groups of a tile, tiles of a sample, pieces of a group wider than a workgroup
+    int splits;                               // chunks of positions of a sample (split)
+    long chunk, blocks;                       // positions of a chunk; workgroups of a tile (resident backward)
+    const void *x, *res, *w, *b, *dy;
+    void *y, *dx, *dres, *dw, *db;
+    float *mean, *rstd, *ws;
+};
+
+struct Plan {
+    Norm d;
+    int threads, k;                           // of the resident kernels; k = 0: split
+};
+
+struct Lane {
+    int vec, group, row, sample;              // vector of its group, group of its tile, first position, sample
+    int dv;                                   // vectors of the group (of this piece)
+    int g, ch;                                // group and first channel within the sample
+    bool live;                                // not padding
+};
+
+template <int V>
+__device__ Lane lane_of(const Norm& d, int tile) {
+    Lane l;
+    const int t = threadIdx.x;
+    l.vec = t & ((1 << d.ldv) - 1);
+    l.group = (t >> d.ldv) & ((1 << d.lgs) - 1);
+    l.row = (t >> (d.ldv + d.lgs)) & ((1 << d.lrows) - 1);
+    l.sample = t >> (d.ldv + d.lgs + d.lrows);
+    l.dv = d.D / V;
+    int first = 0, gs = d.gs;
+    if (d.pieces > 1) {
+        l.g = tile / d.pieces;
+        first = (tile - l.g * d.pieces) << d.ldv;
+        l.dv = l.dv - first < 1 << d.ldv ? l.dv - first : 1 << d.ldv;
+    } else {
+        l.g = tile * d.gs;
+        gs = d.G - l.g < gs ? d.G - l.g : gs;
+    }
+    l.live = l.vec < l.dv && l.group < gs && l.sample < d.samples;
+    if (l.group < gs) l.g += l.group;         // padding reads what a live lane reads, and counts nothing
+    l.ch = l.g * d.D + (first + (l.live ? l.vec : 0)) * V;
+    return l;
+}
+
+// Sums of N values over the lanes of a group (all its vectors and positions, of one sample), to every lane of it.
+// `scratch`: TH * N floats that no thread still reads; an alternation of two needs no barrier in between.
+template <int TH, int N>
+__device__ inline void group_sum(float (&v)[N], const Norm& d, float* scratch) {
+    const int dvp = 1 << d.ldv, pitch = 1 << (d.ldv + d.lgs);
+    for (int m = 1; m < dvp && m < 64; m <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m);
+    for (int m = pitch; m < (pitch << d.lrows) && m < 64; m <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m);
+    if (TH == 64) return;
+    const int t = threadIdx.x, groups = (pitch - 1) & ~(dvp - 1) & ~63;       // bits of the wavefront's number that are a group's
+    // one slot for each group of a wavefront
+    const int slot = (t & 63 & (pitch - 1)) >> (d.ldv < 6 ? d.ldv : 6);
+#pragma unroll
+    for (int k = 0; k < N; ++k) scratch[(t >> 6) * 64 * N + slot * N + k] = v[k];      // lanes of one slot hold the same value
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = 0.f;
+    for (int w = 0; w < TH / 64; ++w)
+        if ((((w << 6) ^ t) & groups) == 0)
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] += scratch[w * 64 * N + slot * N + k];
+}
+
+// Sums of V values over all positions and samples of the workgroup, to the lanes of its first row.  `scratch`: TH * V floats.
+template <int TH, int V>
+__device__ inline void column_sum(float (&v)[V], const Norm& d, float* scratch) {
+    const int pitch = 1 << (d.ldv + d.lgs), t = threadIdx.x;
+    for (int m = pitch; m < 64; m <<= 1)
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += __shfl_xor(v[k], m);
+    if (TH == 64) return;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < V; ++k) scratch[k * TH + t] = v[k];
+    __syncthreads();
+    if (t >= pitch) return;
+    for (int w = 1; w < TH / 64; ++w)
+        if (((w << 6) & (pitch - 1) & ~63) == 0)
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] += scratch[k * TH + (w << 6) + t];
+}
+
+template <typename T>
+__device__ inline float param(const void* p, int f32, int c) {
+    return f32 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
+}
+template <typename T, int V>
+__device__ inline void load_params(const Norm& d, int c, float (&w)[V], float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        w[i] = d.w ? param<T>(d.w, d.params_f32, c + i) : 1.f;
+        b[i] = d.b ? param<T>(d.b, d.params_f32, c + i) : 0.f;
+    }
+}
+
+// No activation and relu share their code: a floor below which z is cut, and a threshold that z has to be above for its slope.
+struct Cut {
+    float floor, edge;
+    __device__ explicit Cut(int act) : floor(act == MZ_ACT_RELU ? 0.f : -INFINITY), edge(act == MZ_ACT_RELU ? 0.f : NAN) {}
+    __device__ float operator()(float z) const { return z < floor ? floor : z; }              // a NaN stays
+    __device__ float slope(float z) const { return z <= edge ? 0.f : 1.f; }
+};
+struct Silu {
+    __device__ explicit Silu(int) {}
+    __device__ float operator()(float z) const { return z / (1.f + __expf(-z)); }
+    __device__ float slope(float z) const {
+        const float s = 1.f / (1.f + __expf(-z));
+        return s * fmaf(z, 1.f - s, 1.f);
+    }
+};
+struct Gelu {
+    __device__ explicit Gelu(int) {}
+    __device__ float operator()(float z) const { return 0.5f * z * (1.f + erff(z * 0.70710678f)); }
+    __device__ float slope(float z) const {
+        return fmaf(z * 0.39894228f, __expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678f)));
+    }
+};
+struct Tanh {
+    __device__ explicit Tanh(int) {}
+    __device__ float operator()(float z) const { return tanhf(z); }
+    __device__ float slope(float z) const {
+        const float t = tanhf(z);
+        return fmaf(-t, t, 1.f);
+    }
+};
+template <typename F>
+__device__ inline void with_activation(int act, F f) {       // the choice is outside the loops over values
+    if (act == MZ_ACT_SILU) f(Silu(act));
+    else if (act == MZ_ACT_GELU) f(Gelu(act));
+    else if (act == MZ_ACT_TANH) f(Tanh(act));
+    else f(Cut(act));
+}
+
+template <typename T, int V, typename A>
+__device__ inline void apply(const Vec<T, V>& x, const Vec<T, V>* res, float mu, float rs, const float (&w)[V], const float (&b)[V],
+                             const A& act, T* y) {
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = fmaf((x[i] - mu) * rs, w[i], b[i]);
+    if (res)
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] += (*res)[i];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = act(f[i]);
+    mz::store<T, V>(y, f);
+}
+
+// h and dz of V values
+template <typename T, int V, typename A>
+__device__ inline void back_values(const Vec<T, V>& x, const Vec<T, V>& dy, const Vec<T, V>* res, float mu, float rs, const float (&w)[V],
+                                   const float (&b)[V], const A& act, float (&h)[V], float (&dz)[V]) {
+    float z[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        h[i] = (x[i] - mu) * rs;
+        z[i] = fmaf(h[i], w[i], b[i]);
+    }
+    if (res)
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] += (*res)[i];
+#pragma unroll
+    for (int i = 0; i < V; ++i) dz[i] = dy[i] * act.slope(z[i]);
+}
+template <typename T, int V>
+__device__ inline void back_store(const Norm& d, long base, unsigned at, float rs, float a, float q, const float (&w)[V], const float (&h)[V],
+                                  float (&dz)[V]) {
+    if (d.dres) mz::store<T, V>(static_cast<T*>(d.dres) + base + at, dz);
+    if (d.dx) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) dz[i] = rs * (fmaf(dz[i], w[i], -a) - h[i] * q);
+        mz::store<T, V>(static_cast<T*>(d.dx) + base + at, dz);
+    }
+}
+
+// ---- resident ---------------------------------------------------------------------------------------------------------
+
+// Up to K vectors a thread, positions row, row + step, ...: addresses are a workgroup's base and 32-bit byte offsets (the host
+// checks that they suffice), a scalar base and one register a vector.
+template <typename T, int V, int K>
+__device__ inline void load_rows(Vec<T, V> (&v)[K], const T* base, int at, int stride, int row, int step, int S) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (k * step < S) {                                 // the same for every thread
+            const int s = row + k * step < S ? row + k * step : S - 1;      // past the end the last again, which counts nothing
+            const unsigned bytes = (unsigned)(at + s * stride) * (unsigned)sizeof(T);
+            v[k] = *reinterpret_cast<const Vec<T, V>*>(reinterpret_cast<const char*>(base) + bytes);
+        }
+}
+
+// Ends what the compiler knows of loaded values, so that what is computed from them after the sums is computed anew: kept,
+// the converted values, h and dz would take several times the registers of the vectors themselves.
+template <typename T, int V, int K>
+__device__ inline void forget(Vec<T, V> (&v)[K]) {
+    if constexpr (sizeof(T) * V >= 4)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < Vec<T, V>::kWords; ++i) {
+                uint32_t w = v[k].w[i];
+                asm volatile("" : "+v"(w));
+                v[k].w[i] = w;
+            }
+}
+
+template <typename T, int V, int TH, int K>
+__global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
+    __shared__ float scratch[2][TH];
+    const int S = (int)d.S, step = 1 << d.lrows;
+    const float inv = 1.f / ((float)d.S * (float)d.D);
+    const long units = (d.N + d.samples - 1) / d.samples * d.tiles;
+    for (long unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const long set = unit / d.tiles, n0 = set * d.samples;
+        const Lane l = lane_of<V>(d, (int)(unit - set * d.tiles));
+        const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;       // samples of this workgroup
+        const bool live = l.live && l.sample < left;
+        const int j = live ? l.sample : 0;
+        Vec<T, V> xv[K], rv[K];
+        load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
+        if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
+        float w[V], b[V];
+        load_params<T, V>(d, l.ch, w, b);
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k * step < S) {
+                float p = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) p += xv[k][i];
+                sum[0] += live && l.row + k * step < S ? p : 0.f;
+            }
+        group_sum<TH>(sum, d, scratch[0]);
+        const float mu = sum[0] * inv;
+        sum[0] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k * step < S) {
+                float p = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) p = fmaf(xv[k][i] - mu, xv[k][i] - mu, p);
+                sum[0] += live && l.row + k * step < S ? p : 0.f;
+            }
+        group_sum<TH>(sum, d, scratch[1]);
+        const float rs = 1.f / sqrtf(sum[0] * inv + d.eps);
+        if (!live) continue;
+        if (d.mean && l.vec == 0 && l.row == 0) {
+            d.mean[(n0 + j) * d.G + l.g] = mu;
+            d.rstd[(n0 + j) * d.G + l.g] = rs;
+        }
+        T* y = static_cast<T*>(d.y) + n0 * d.S * d.C;
+        const int at = (j * S + l.row) * d.C + l.ch;
+        with_activation(d.act, [&](auto act) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (l.row + k * step < S)
+                    apply<T, V>(xv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, y + (unsigned)(at + k * step * d.C));
+        });
+    }
+}
+
+// A workgroup keeps its tile and strides over the samples: the channels' sums for dweight and dbias stay in registers and
+// leave one row of ws [blocks][2][C] a workgroup.
+template <typename T, int V, int TH, int K>
+__global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
+    __shared__ float scratch[TH == 64 ? 1 : TH * (V > 2 ? 2 * V : 4)];
+    const int S = (int)d.S, step = 1 << d.lrows;
+    const float inv = 1.f / ((float)d.S * (float)d.D);
+    const long block = blockIdx.x / d.tiles;
+    const Lane l = lane_of<V>(d, (int)(blockIdx.x - block * d.tiles));
+    float w[V], b[V], s1[V] = {}, s2[V] = {};
+    load_params<T, V>(d, l.ch, w, b);
+    int turn = 0;
+    for (long n0 = block * d.samples; n0 < d.N; n0 += d.blocks * d.samples, turn ^= 1) {
+        const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;
+        const bool live = l.live && l.sample < left;
+        const int j = live ? l.sample : 0;
+        Vec<T, V> xv[K], gv[K], rv[K];
+        load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
+        load_rows<T, V, K>(gv, static_cast<const T*>(d.dy) + n0 * d.ds[0], j * (int)d.ds[0] + l.ch, (int)d.ds[1], l.row, step, S);
+        if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
+        const float mu = d.mean[(n0 + j) * d.G + l.g], rs = d.rstd[(n0 + j) * d.G + l.g];
+        float aq[2] = {0.f, 0.f};
+        with_activation(d.act, [&](auto act) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!live || l.row + k * step >= S) continue;
+                float h[V], dz[V];
+                back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    s1[i] += dz[i];
+                    s2[i] = fmaf(dz[i], h[i], s2[i]);
+                    aq[0] = fmaf(dz[i], w[i], aq[0]);
+                    aq[1] = fmaf(dz[i] * w[i], h[i], aq[1]);
+                }
+            }
+        });
+        group_sum<TH>(aq, d, TH == 64 ? scratch : scratch + turn * 2 * TH);
+        const float a = aq[0] * inv, q = aq[1] * inv;
+        const long out = n0 * d.S * d.C;
+        const int at = (j * S + l.row) * d.C + l.ch;
+        forget(xv);
+        forget(gv);
+        forget(rv);
+        with_activation(d.act, [&](auto act) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!live || l.row + k * step >= S) continue;
+                float h[V], dz[V];
+                back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
+                back_store<T, V>(d, out, (unsigned)(at + k * step * d.C), rs, a, q, w, h, dz);
+            }
+        });
+    }
+    if (!d.dw && !d.db) return;
+    column_sum<TH>(s1, d, scratch);
+    column_sum<TH>(s2, d, TH == 64 ? scratch : scratch + TH * V);
+    if (l.live && l.row == 0 && l.sample == 0) {
+        float* ws = d.ws + block * 2 * d.C + l.ch;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            ws[i] = s1[i];
+            ws[d.C + i] = s2[i];
+        }
+    }
+}
+
+// ---- split ------------------------------------------------------------------------------------------------------------
+
+struct Part {
+    long n, s0, s1;
+    int split, tile;
+};
+__device__ inline Part part_of(const Norm& d, long id) {
+    Part p;
+    p.tile = (int)(id % d.tiles);
+    id /= d.tiles;
+    p.split = (int)(id % d.splits);
+    p.n = id / d.splits;
+    p.s0 = p.split * d.chunk;
+    p.s1 = p.s0 + d.chunk < d.S ? p.s0 + d.chunk : d.S;
+    return p;
+}
+// where (split, piece) of a group stands among its splits * pieces partial results
+__device__ inline long part_at(const Norm& d, const Part& p, const Lane& l) {
+    return ((p.n * d.G + l.g) * d.splits + p.split) * d.pieces + (d.pieces > 1 ? p.tile % d.pieces : 0);
+}
+
+// ws [N][G][splits][pieces][2]: mean and sum of squared deviations of each part
+template <typename T, int V>
+__global__ void __launch_bounds__(kSplitThreads) norm_stats_kernel(Norm d) {
+    __shared__ float scratch[2][kSplitThreads];
+    const int step = 1 << d.lrows;
+    const long total = d.N * d.tiles * d.splits;
+    for (long id = blockIdx.x; id < total; id += gridDim.x) {
+        const Part p = part_of(d, id);
+        const Lane l = lane_of<V>(d, p.tile);
+        float count = 0.f, mean = 0.f, m2 = 0.f;
+        if (l.live) {
+            const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
+            constexpr int U = 4;
+            for (long s = p.s0 + l.row; s < p.s1; s += U * step) {     // U vectors on their own, then merged
+                Vec<T, V> v[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) v[k] = mz::load<T, V>(x + (s + k * step < p.s1 ? s + k * step : s) * d.xs[1]);
+                float sum = 0.f, more = 0.f, dev = 0.f;
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const bool in = s + k * step < p.s1;
+                    more += in ? (float)V : 0.f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum += in ? v[k][i] : 0.f;
+                }
+                const float m = sum / more;
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float e = s + k * step < p.s1 ? v[k][i] - m : 0.f;
+                        dev = fmaf(e, e, dev);
+                    }
+                const float e = m - mean, f = more / (count + more);
+                mean = fmaf(e, f, mean);
+                m2 += dev + e * e * count * f;
+                count += more;
+            }
+        }
+        const float all = (float)(p.s1 - p.s0) * (float)(l.dv * V);
+        float v[1] = {count * mean};
+        group_sum<kSplitThreads>(v, d, scratch[0]);
+        const float mu = v[0] / all;
+        v[0] = count > 0.f ? fmaf(count * (mean - mu), mean - mu, m2) : 0.f;
+        group_sum<kSplitThreads>(v, d, scratch[1]);
+        if (l.live && l.vec == 0 && l.row == 0) {
+            float* ws = d.ws + 2 * part_at(d, p, l);
+            ws[0] = mu;
+            ws[1] = v[0];
+        }
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kSplitThreads) norm_apply_kernel(Norm d) {
+    __shared__ float scratch[2][kSplitThreads];
+    const int step = 1 << d.lrows;
+    const float inv = 1.f / ((float)d.S * (float)d.D);
+    const long total = d.N * d.tiles * d.splits;
+    for (long id = blockIdx.x; id < total; id += gridDim.x) {
+        const Part p = part_of(d, id);
+        const Lane l = lane_of<V>(d, p.tile);
+        const long ng = p.n * d.G + l.g;
+        // the group's parts, over its lanes (a part's share of the values: its positions times its vectors)
+        const float* ws = d.ws + 2 * ng * d.splits * d.pieces;
+        const int parts = d.splits * d.pieces, lanes = 1 << (d.ldv + d.lrows), mine = (l.row << d.ldv) + l.vec;
+        const auto count = [&](int e) {
+            const int split = e / d.pieces, piece = e - split * d.pieces, left = d.D / V - (piece << d.ldv);
+            const long positions = split * d.chunk + d.chunk < d.S ? d.chunk : d.S - split * d.chunk;
+            return (float)positions * (float)((left < 1 << d.ldv ? left : 1 << d.ldv) * V);
+        };
+        float v[1] = {0.f};
+        if (l.group < d.gs)
+            for (int e = mine; e < parts; e += lanes) v[0] = fmaf(count(e), ws[2 * e], v[0]);
+        group_sum<kSplitThreads>(v, d, scratch[0]);
+        const float mu = v[0] * inv;
+        v[0] = 0.f;
+        if (l.group < d.gs)
+            for (int e = mine; e < parts; e += lanes) v[0] += fmaf(count(e) * (ws[2 * e] - mu), ws[2 * e] - mu, ws[2 * e + 1]);
+        group_sum<kSplitThreads>(v, d, scratch[1]);
+        const float rs = 1.f / sqrtf(v[0] * inv + d.eps);
+        if (!l.live) continue;
+        if (d.mean && p.split == 0 && l.vec == 0 && l.row == 0 && (d.pieces == 1 || p.tile % d.pieces == 0)) {
+            d.mean[ng] = mu;
+            d.rstd[ng] = rs;
+        }
+        float w[V], b[V];
+        load_params<T, V>(d, l.ch, w, b);
+        const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
+        const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
+        T* y = static_cast<T*>(d.y) + p.n * d.S * d.C + l.ch;
+        with_activation(d.act, [&](auto act) {
+            constexpr int U = 4;
+            for (long s = p.s0 + l.row; s < p.s1; s += U * step) {
+                Vec<T, V> v[U], r[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const long at = s + k * step < p.s1 ? s + k * step : s;
+                    v[k] = mz::load<T, V>(x + at * d.xs[1]);
+                    if (res) r[k] = mz::load<T, V>(res + at * d.rs[1]);
+                }
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (s + k * step < p.s1) apply<T, V>(v[k], res ? &r[k] : nullptr, mu, rs, w, b, act, y + (s + k * step) * d.C);
+            }
+        });
+    }
+}
+
+// ws: sums of dz and dz h of a chunk's positions, [N * splits][2][C], then sums of dz w and dz w h of each part,
+// [N][G][splits][pieces][2]
+template <typename T, int V>
+__global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
+    __shared__ float scratch[2][kSplitThreads * (V > 2 ? V : 2)];
+    const int step = 1 << d.lrows;
+    const long total = d.N * d.tiles * d.splits;
+    for (long id = blockIdx.x; id < total; id += gridDim.x) {
+        const Part p = part_of(d, id);
+        const Lane l = lane_of<V>(d, p.tile);
+        const long ng = p.n * d.G + l.g;
+        float s1[V] = {}, s2[V] = {}, w[V], b[V];
+        load_params<T, V>(d, l.ch, w, b);
+        if (l.live) {
+            const float mu = d.mean[ng], rs = d.rstd[ng];
+            const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
+            const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
+            const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
+            with_activation(d.act, [&](auto act) {
+                constexpr int U = 4;
+                for (long s = p.s0 + l.row; s < p.s1; s += U * step) {
+                    Vec<T, V> v[U], g[U], r[U];
+#pragma unroll
+                    for (int k = 0; k < U; ++k) {
+                        const long at = s + k * step < p.s1 ? s + k * step : s;
+                        v[k] = mz::load<T, V>(x + at * d.xs[1]);
+                        g[k] = mz::load<T, V>(dy + at * d.ds[1]);
+                        if (res) r[k] = mz::load<T, V>(res + at * d.rs[1]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < U; ++k) {
+                        if (s + k * step >= p.s1) continue;
+                        float h[V], dz[V];
+                        back_values<T, V>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            s1[i] += dz[i];
+                            s2[i] = fmaf(dz[i], h[i], s2[i]);
+                        }
+                    }
+                }
+            });
+        }
+        float aq[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            aq[0] = fmaf(s1[i], w[i], aq[0]);
+            aq[1] = fmaf(s2[i], w[i], aq[1]);
+        }
+        __syncthreads();
+        group_sum<kSplitThreads>(aq, d, scratch[0]);
+        column_sum<kSplitThreads>(s1, d, scratch[1]);
+        column_sum<kSplitThreads>(s2, d, scratch[0]);
+        if (l.live && l.row == 0) {
+            float* ws = d.ws + (p.n * d.splits + p.split) * 2 * d.C + l.ch;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                ws[i] = s1[i];
+                ws[d.C + i] = s2[i];
+            }
+            if (l.vec == 0) {
+                float* at = d.ws + d.N * d.splits * 2 * d.C + 2 * part_at(d, p, l);
+                at[0] = aq[0];
+                at[1] = aq[1];
+            }
+        }
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) {
+    __shared__ float scratch[2][2 * kSplitThreads];
+    const int step = 1 << d.lrows;
+    const float inv = 1.f / ((float)d.S * (float)d.D);
+    const long total = d.N * d.tiles * d.splits;
+    int turn = 0;
+    for (long id = blockIdx.x; id < total; id += gridDim.x, turn ^= 1) {
+        const Part p = part_of(d, id);
+        const Lane l = lane_of<V>(d, p.tile);
+        const long ng = p.n * d.G + l.g;
+        const float* ws = d.ws + d.N * d.splits * 2 * d.C + 2 * ng * d.splits * d.pieces;
+        float aq[2] = {0.f, 0.f};
+        if (l.group < d.gs)
+            for (int e = (l.row << d.ldv) + l.vec; e < d.splits * d.pieces; e += 1 << (d.ldv + d.lrows)) {
+                aq[0] += ws[2 * e];
+                aq[1] += ws[2 * e + 1];
+            }
+        group_sum<kSplitThreads>(aq, d, scratch[turn]);
+        if (!l.live) continue;
+        const float mu = d.mean[ng], rs = d.rstd[ng], a = aq[0] * inv, q = aq[1] * inv;
+        float w[V], b[V];
+        load_params<T, V>(d, l.ch, w, b);
+        const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
+        const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
+        const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
+        const long out = p.n * d.S * d.C + l.ch;
+        with_activation(d.act, [&](auto act) {
+            constexpr int U = 4;
+            for (long s = p.s0 + l.row; s < p.s1; s += U * step) {
+                Vec<T, V> v[U], g[U], r[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const long at = s + k * step < p.s1 ? s + k * step : s;
+                    v[k] = mz::load<T, V>(x + at * d.xs[1]);
+                    g[k] = mz::load<T, V>(dy + at * d.ds[1]);
+                    if (res) r[k] = mz::load<T, V>(res + at * d.rs[1]);
+                }
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    if (s + k * step >= p.s1) continue;
+                    float h[V], dz[V];
+                    back_values<T, V>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
+                    back_store<T, V>(d, out + (s + k * step) * d.C, 0, rs, a, q, w, h, dz);
+                }
+            }
+        });
+    }
+}
+
+// ---- dweight, dbias ---------------------------------------------------------------------------------------------------
+
+// ws [rows][2][C] summed over its rows: 16 columns a workgroup, 64 rows side by side, in 64 bits (sums over every position
+// of a batch, which may cancel)
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_params_kernel(Norm d, long rows) {
+    __shared__ double part[1024];
+    const int t = threadIdx.x, c = blockIdx.x * 16 + (t & 15);
+    double s = 0.0;
+    if (c < 2 * d.C)
+        for (long r = t >> 4; r < rows; r += 64) s += d.ws[r * 2 * d.C + c];
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    part[t] = s;
+    __syncthreads();
+    if (t < 16 && c < 2 * d.C) {
+        for (int j = 1; j < 16; ++j) s += part[j * 64 + t];
+        const bool which = c >= d.C;
+        void* out = which ? d.dw : d.db;
+        const int at = which ? c - d.C : c;
+        if (!out) return;
+        if (d.params_f32) static_cast<float*>(out)[at] = (float)s;
+        else static_cast<T*>(out)[at] = (T)(float)s;
+    }
+}
+
+// ---- launches, one file a type ----------------------------------------------------------------------------------------
+
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+template <typename T, typename F>
+void with_vector(int v, F f) {
+    if constexpr (sizeof(T) == 2)
+        if (v == 8) return f(Int<8>{});
+    if (v == 4) f(Int<4>{});
+    else if (v == 2) f(Int<2>{});
+    else f(Int<1>{});
+}
+template <typename F>
+void with_size(const Plan& p, F f) {                // threads, and vectors a thread, of the resident kernels
+    if (p.threads == 64) {
+        if (p.k <= 2) f(Int<64>{}, Int<2>{});
+        else f(Int<64>{}, Int<8>{});
+    } else if (p.threads == 256) {
+        f(Int<256>{}, Int<8>{});
+    } else {
+        f(Int<512>{}, Int<8>{});
+    }
+}
+inline unsigned grid_of(long total) { return (unsigned)(total < (1L << 22) ? total : 1L << 22); }
+
+template <typename T>
+void forward(const Plan& p, int v, hipStream_t st) {
+    const Norm& d = p.d;
+    with_vector<T>(v, [&](auto v_) {
+        constexpr int V = v_.value;
+        if (p.k) {
+            const unsigned grid = grid_of((d.N + d.samples - 1) / d.samples * d.tiles);
+            with_size(p, [&](auto th, auto k) { norm_forward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
+        } else {
+            const unsigned grid = grid_of(d.N * d.tiles * d.splits);
+            norm_stats_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
+            norm_apply_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
+        }
+    });
+}
+
+template <typename T>
+void backward(const Plan& p, int v, hipStream_t st) {
+    const Norm& d = p.d;
+    const bool empty = d.N == 0 || d.S == 0;
+    if (!empty)
+        with_vector<T>(v, [&](auto v_) {
+            constexpr int V = v_.value;
+            if (p.k) {
+                const unsigned grid = (unsigned)(d.blocks * d.tiles);
+                with_size(p, [&](auto th, auto k) { norm_backward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
+            } else {
+                const unsigned grid = grid_of(d.N * d.tiles * d.splits);
+                norm_back_sums_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
+                if (d.dx || d.dres) norm_back_apply_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
+            }
+        });
+    if (d.dw || d.db)           // of no rows: zeros
+        norm_params_kernel<T><<<(2 * d.C + 15) / 16, 1024, 0, st>>>(d, empty ? 0 : p.k ? d.blocks : d.N * d.splits);
+}
+
+extern template void forward<float>(const Plan&, int, hipStream_t);
+extern template void forward<mz::f16>(const Plan&, int, hipStream_t);
+extern template void forward<mz::bf16>(const Plan&, int, hipStream_t);
+extern template void backward<float>(const Plan&, int, hipStream_t);
+extern template void backward<mz::f16>(const Plan&, int, hipStream_t);
+extern template void backward<mz::bf16>(const Plan&, int, hipStream_t);
+
+}  // namespace mz_norm

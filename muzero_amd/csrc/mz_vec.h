@@ -1,6 +1,8 @@
 // Element types, vector loads and reductions of the training operators (mz_norm.hip, mz_loss.hip, mz_clip.hip).
 #pragma once
 #include "mz_common.h"
+#include <cstdint>
+#include <type_traits>
 
 namespace mz {
 
@@ -9,11 +11,21 @@ typedef __bf16 bf16;
 
 inline int dtype_size(int dtype) { return dtype == MZ_F32 ? 4 : dtype == MZ_F16 || dtype == MZ_BF16 ? 2 : 0; }
 
-// V elements that are loaded and stored as one access.  Aligned like ONE element: gfx950 takes a 4-, 8- or 16-byte access at
-// any element address, so rows of odd widths and views at odd offsets keep their wide accesses.
+// V elements that are loaded and stored as one access, kept as they lie in memory: 16-bit elements stay two to a register
+// until they are used.  Aligned like ONE element: gfx950 takes a 4-, 8- or 16-byte access at any element address, so rows of
+// odd widths and views at odd offsets keep their wide accesses.
 template <typename T, int V>
 struct __attribute__((packed, aligned(sizeof(T)))) Vec {
-    T v[V];
+    typedef typename std::conditional<sizeof(T) * V >= 4, uint32_t, uint16_t>::type Word;
+    static constexpr int kWords = sizeof(T) * V / sizeof(Word);
+    Word w[kWords];
+
+    __device__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[i]);
+        else if constexpr (V == 1) return (float)__builtin_bit_cast(T, w[0]);
+        else if constexpr (std::is_same<T, bf16>::value) return __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else return (float)__builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (i & 1) * 16));
+    }
 };
 
 template <typename T, int V>
@@ -21,11 +33,15 @@ __device__ inline Vec<T, V> load(const T* p) {
     return *reinterpret_cast<const Vec<T, V>*>(p);
 }
 template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Elements {
+    T v[V];
+};
+template <typename T, int V>
 __device__ inline void store(T* p, const float (&f)[V]) {
-    Vec<T, V> r;
+    Elements<T, V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = (T)f[i];       // one rounding to the stored type, to nearest even
-    *reinterpret_cast<Vec<T, V>*>(p) = r;
+    *reinterpret_cast<Elements<T, V>*>(p) = r;
 }
 
 template <typename T>
