@@ -6,6 +6,9 @@ from .exceptions import MuZeroError
 
 DTYPES = {torch.float32: _lib.MZ_F32, torch.float16: _lib.MZ_F16, torch.bfloat16: _lib.MZ_BF16}
 
+# the current stream's handle; the call behind torch.cuda.current_stream, which takes 25 times as long to wrap it
+_current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 _ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros((), requires_grad=True)).node)
 
 
@@ -27,13 +30,21 @@ def require_hip(device):
 
 def launch(device, fn, *args):
     """fn(stream, *args) of libmzhip.so on `device`'s current stream, with that device current."""
-    if device.index == torch.cuda.current_device():
-        status = fn(torch.cuda.current_stream(device).cuda_stream, *args)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(_current_stream(index), *args)
     else:
         with torch.cuda.device(device):
-            status = fn(torch.cuda.current_stream(device).cuda_stream, *args)
+            status = fn(_current_stream(index), *args)
     if status < 0:
         _lib.check(status)
+
+
+def once(backward):
+    """backward of an autograd.Function that is differentiable once: the usual pass runs with gradients off and goes straight
+    through; under create_graph=True its results refuse to be differentiated again."""
+    refusing = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
 def refuse_capture_of_live_leaves(device, tensors):
@@ -42,7 +53,7 @@ def refuse_capture_of_live_leaves(device, tensors):
     capture, which ends the process: refused here, before anything is captured."""
     if not torch.cuda.is_current_stream_capturing():
         return
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = _current_stream(device.index)
     for t in tensors:
         if t is not None and t.requires_grad and t.is_leaf:
             made_on = torch.autograd.graph.get_gradient_edge(t).node.metadata.get('mzhip_stream', stream)
@@ -55,5 +66,5 @@ def remember_leaves(device, output):
     """Notes the stream on the accumulation nodes of `output`'s leaves, for refuse_capture_of_live_leaves."""
     for node, _ in output.grad_fn.next_functions:
         if type(node) is _ACCUMULATE and 'mzhip_stream' not in node.metadata:
-            node.metadata['mzhip_stream'] = torch.cuda.current_stream(device).cuda_stream
+            node.metadata['mzhip_stream'] = _current_stream(device.index)
     return output

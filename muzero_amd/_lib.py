@@ -149,10 +149,11 @@ PROTOTYPES = {
                                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     'mz_selfplay_step_record': (ctypes.c_int, [c_void_p, ctypes.POINTER(Env), ctypes.POINTER(History)] + [c_void_p] * 6),
     'mz_replay_targets': (ctypes.c_int, [c_void_p, ctypes.POINTER(ReplayConfig)] + [c_void_p] * 12),
-    'mz_group_norm_workspace': (c_int64, [ctypes.POINTER(GroupNorm), c_int32]),
-    'mz_group_norm_forward': (ctypes.c_int, [c_void_p, ctypes.POINTER(GroupNorm)] + [c_void_p] * 8 + [c_int64]),
-    'mz_group_norm_backward': (ctypes.c_int, [c_void_p, ctypes.POINTER(GroupNorm)] + [c_void_p] * 12 + [c_int64]),
-    'mz_categorical_loss': (ctypes.c_int, [c_void_p, ctypes.POINTER(Categorical)] + [c_void_p] * 8),
+    # the configurations of the training operators: a structure by reference, or its bytes
+    'mz_group_norm_workspace': (c_int64, [c_void_p, c_int32]),
+    'mz_group_norm_forward': (ctypes.c_int, [c_void_p, c_void_p] + [c_void_p] * 8 + [c_int64]),
+    'mz_group_norm_backward': (ctypes.c_int, [c_void_p, c_void_p] + [c_void_p] * 12 + [c_int64]),
+    'mz_categorical_loss': (ctypes.c_int, [c_void_p, c_void_p] + [c_void_p] * 8),
     'mz_global_norm': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
     'mz_clip_by_global_norm': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_double, c_void_p, c_int64, c_void_p]),
     'mz_env_cartpole_step': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -1,107 +1,108 @@
 """Layers of networks composed outside the built-in kernels, next to network.py's state-action encoders: group norm with
 an activation over channels-last states (csrc/mz_norm.hip), forward and backward."""
-import ctypes
+import functools
 import math
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from ._launch import DTYPES, launch, refuse_capture_of_live_leaves, remember_leaves, require_hip, require_tensor
+from ._launch import DTYPES, launch, refuse_capture_of_live_leaves, once, remember_leaves, require_hip, require_tensor
 from .exceptions import MuZeroError
 
 ACTIVATIONS = {None: _lib.MZ_ACT_NONE, 'relu': _lib.MZ_ACT_RELU, 'silu': _lib.MZ_ACT_SILU, 'gelu': _lib.MZ_ACT_GELU,
                'tanh': _lib.MZ_ACT_TANH}
 
 
+# mz_group_norm_t up to its dy_strides, and those
+_CONFIG, _DY = struct.Struct('=qqiiiiiidqqqq'), struct.Struct('=qq')
+
+
 def _states(t):
     """-> (t or a dense copy of it, batch stride, position stride): the kernels walk a state as [batch][positions][C] with
     adjacent channels and one stride each for batch and positions."""
-    shape, stride = t.shape, t.stride()
-    if t.is_contiguous():
-        c = shape[-1]
-        return t, t.numel() // max(shape[0], 1), c
-    if stride[-1] == 1 or shape[-1] == 1:
-        step, span, ok = 0, 1, True
-        for size, st in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
-            if size == 1:
-                continue
-            if span == 1:
-                step = st
-            ok &= st == step * span
-            span *= size
-        if ok:
-            return t, stride[0], step
-    return t.contiguous(), math.prod(shape[1:]), shape[-1]
+    shape = t.shape
+    if not t.is_contiguous():
+        stride = t.stride()
+        if stride[-1] == 1 or shape[-1] == 1:
+            step, span, ok = 0, 1, True
+            for size, st in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
+                if size == 1:
+                    continue
+                if span == 1:
+                    step = st
+                ok &= st == step * span
+                span *= size
+            if ok:
+                return t, stride[0], step
+        t = t.contiguous()
+    return t, math.prod(shape[1:]), shape[-1]
 
 
-def _describe(x, groups, param_dtype, activation, eps, residual, dy=None):
-    cfg = _lib.GroupNorm()
-    cfg.batch, cfg.channels, cfg.groups = x.shape[0], x.shape[-1], groups
-    cfg.positions = math.prod(x.shape[1:-1])
-    cfg.dtype, cfg.param_dtype, cfg.activation, cfg.eps = DTYPES[x.dtype], DTYPES[param_dtype], activation, eps
-    x, cfg.x_strides[0], cfg.x_strides[1] = _states(x)
-    if residual is not None:
-        residual, cfg.residual_strides[0], cfg.residual_strides[1] = _states(residual)
-    if dy is not None:
-        dy, cfg.dy_strides[0], cfg.dy_strides[1] = _states(dy)
-    return cfg, x, residual, dy
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(config, backward):
+    n = _lib.load().mz_group_norm_workspace(config, backward)
+    if n < 0:
+        _lib.check(n)
+    return n
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(lib, cfg, backward, device):
-    n = lib.mz_group_norm_workspace(ctypes.byref(cfg), backward)
-    if n < 0:
-        _lib.check(n)
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None, n
-
-
 def _forward(x, groups, weight, bias, eps, activation, residual, statistics):
-    lib = _lib.load()
-    cfg, xs, rs, _ = _describe(x, groups, _param_dtype(x, weight, bias), activation, eps, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
+    """-> y, mean and rstd [2, B, groups] or None, x and residual as the kernels read them, the configuration."""
+    shape, dtype, device = x.shape, x.dtype, x.device
+    x, xb, xp = _states(x)
+    rb = rp = 0
+    if residual is not None:
+        residual, rb, rp = _states(residual)
+    param = weight if weight is not None else bias
+    config = _CONFIG.pack(shape[0], math.prod(shape[1:-1]), shape[-1], groups, DTYPES[dtype],
+                          _lib.MZ_F32 if param is None else DTYPES[param.dtype], activation, 0, eps, xb, xp, rb, rp)
+    y = torch.empty(shape, dtype=dtype, device=device)
+    stats = mean = rstd = None
     if statistics:
-        mean, rstd = torch.empty(2, x.shape[0], groups, dtype=torch.float32, device=x.device)
-    ws, n = _workspace(lib, cfg, 0, x.device)
-    launch(x.device, lib.mz_group_norm_forward, ctypes.byref(cfg), xs.data_ptr(), _ptr(rs), _ptr(weight), _ptr(bias),
-           y.data_ptr(), _ptr(mean), _ptr(rstd), _ptr(ws), n)
-    return y, mean, rstd
-
-
-def _param_dtype(x, weight, bias):
-    return weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+        stats = torch.empty(2, shape[0], groups, dtype=torch.float32, device=device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * shape[0] * groups
+    whole = config + _DY.pack(0, 0)
+    n = _workspace_bytes(whole, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    launch(device, _lib.load().mz_group_norm_forward, whole, x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), y.data_ptr(),
+           mean, rstd, _ptr(ws), n)
+    return y, stats, x, residual, config
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, groups, eps, activation):
-        y, mean, rstd = _forward(x, groups, weight, bias, eps, activation, residual, True)
+        y, stats, x, residual, config = _forward(x, groups, weight, bias, eps, activation, residual, True)
         # the residual enters the gradients through the activation's argument alone
-        ctx.save_for_backward(x, weight, bias, residual if activation else None, mean, rstd)
-        ctx.rest = groups, eps, activation
+        ctx.save_for_backward(x, weight, bias, residual if activation else None, stats)
+        ctx.config = config
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy):
-        x, weight, bias, residual, mean, rstd = ctx.saved_tensors
-        groups, eps, activation = ctx.rest
+        x, weight, bias, residual, stats = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        lib = _lib.load()
-        cfg, xs, rs, dys = _describe(x, groups, _param_dtype(x, weight, bias), activation, eps, residual, dy)
-        new = lambda like: torch.empty(like.shape, dtype=like.dtype, device=like.device)
-        dx = new(x) if need_x else None
-        dres = new(x) if need_r else None
-        dw = new(weight) if need_w else None
-        db = new(bias) if need_b else None
-        ws, n = _workspace(lib, cfg, 1, x.device)
-        launch(x.device, lib.mz_group_norm_backward, ctypes.byref(cfg), xs.data_ptr(), _ptr(rs), _ptr(weight), _ptr(bias),
-               mean.data_ptr(), rstd.data_ptr(), dys.data_ptr(), _ptr(dx), _ptr(dres), _ptr(dw), _ptr(db), _ptr(ws), n)
-        return dx, dw, db, dres, None, None, None
+        dy, db, dp = _states(dy)
+        config = ctx.config + _DY.pack(db, dp)
+        device = x.device
+        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+        dres = torch.empty(x.shape, dtype=x.dtype, device=device) if need_r else None
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=device) if need_w else None
+        dbias = torch.empty(bias.shape, dtype=bias.dtype, device=device) if need_b else None
+        n = _workspace_bytes(config, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        mean = stats.data_ptr()
+        launch(device, _lib.load().mz_group_norm_backward, config, x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), mean,
+               mean + stats.numel() * 2, dy.data_ptr(), _ptr(dx), _ptr(dres), _ptr(dw), _ptr(dbias), _ptr(ws), n)
+        return dx, dw, dbias, dres, None, None, None
 
 
 def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -139,8 +140,9 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     act = ACTIVATIONS[activation]
-    tensors = (x, weight, bias, residual)
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled() or not (x.requires_grad or weight is not None and weight.requires_grad
+                                           or bias is not None and bias.requires_grad
+                                           or residual is not None and residual.requires_grad):
         return _forward(x, num_groups, weight, bias, eps, act, residual, False)[0]
-    refuse_capture_of_live_leaves(device, tensors)
+    refuse_capture_of_live_leaves(device, (x, weight, bias, residual))
     return remember_leaves(device, _GroupNorm.apply(x, weight, bias, residual, num_groups, eps, act))

@@ -3,109 +3,113 @@ global gradient norm and clipping by it (csrc/mz_clip.hip).  The reference leave
 the names follow its framework."""
 import ctypes
 import math
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from ._launch import DTYPES, launch, refuse_capture_of_live_leaves, remember_leaves, require_hip, require_tensor
+from ._launch import DTYPES, launch, once, refuse_capture_of_live_leaves, remember_leaves, require_hip, require_tensor
 from .exceptions import MuZeroError
 
 MAX_CLASSES = 4096
 
 
 # ---- categorical loss ----------------------------------------------------------------------------------------------------
-class _LossCall:
-    """The checked arguments of one loss: [unroll, batch] rows with a stride for each."""
+# mz_categorical_t up to its dloss_strides, and those
+_CONFIG, _DLOSS = struct.Struct('=qqqqiiiiqqqq'), struct.Struct('=qq')
 
-    def __init__(self, logits, targets, game, position, weights):
-        require_tensor('logits', logits, DTYPES)
-        device = self.device = logits.device
-        if logits.dim() < 2 or not 1 <= logits.shape[-1] <= MAX_CLASSES:
-            raise MuZeroError(f'logits must be [..., classes] with 1 to {MAX_CLASSES} classes, got {tuple(logits.shape)}')
-        require_tensor('targets', targets, (torch.float32,), device)
-        if targets.requires_grad:
-            raise MuZeroError('the loss is not differentiable with respect to targets')
-        indexed = game is not None or position is not None
-        if indexed:
-            if logits.dim() != 3:
-                raise MuZeroError(f'with game and position, logits must be [unroll, batch, classes], got {tuple(logits.shape)}')
-            if game is None or position is None:
-                raise MuZeroError('game and position: both or neither')
-            if targets.dim() != 3 or targets.shape[-1] != logits.shape[-1]:
-                raise MuZeroError(f'targets must be [positions, games, {logits.shape[-1]}], got {tuple(targets.shape)}')
-            for name, t in (('game', game), ('position', position)):
-                require_tensor(name, t, (torch.int32, torch.int64), device)
-                if t.shape != logits.shape[1:2]:
-                    raise MuZeroError(f'{name} must have shape ({logits.shape[1]},), got {tuple(t.shape)}')
-            if game.dtype != position.dtype:
-                raise MuZeroError(f'game is {game.dtype}, position {position.dtype}: both must be of one type')
-        elif targets.shape != logits.shape:
-            raise MuZeroError(f'targets have shape {tuple(targets.shape)}, logits {tuple(logits.shape)}')
-        self.shape = logits.shape[:-1]
-        if weights is not None:
-            require_tensor('weights', weights, (torch.float32,), device)
-            if weights.requires_grad:
-                raise MuZeroError('the loss is not differentiable with respect to weights')
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t):
+    """A tensor of the rows' shape -> (t or a dense copy of it, unroll stride, batch stride)."""
+    if t.dim() == 2:
+        return (t, *t.stride())
+    return t.contiguous(), 0, 1
+
+
+def _describe(logits, targets, game, position, weights):
+    """Checks the arguments of a loss -> the tensors as the kernel reads them (logits, targets, game, position, weights) and
+    the configuration without dloss_strides."""
+    require_tensor('logits', logits, DTYPES)
+    device, shape = logits.device, logits.shape
+    if len(shape) < 2 or not 1 <= shape[-1] <= MAX_CLASSES:
+        raise MuZeroError(f'logits must be [..., classes] with 1 to {MAX_CLASSES} classes, got {tuple(shape)}')
+    require_tensor('targets', targets, (torch.float32,), device)
+    if targets.requires_grad:
+        raise MuZeroError('the loss is not differentiable with respect to targets')
+    rows, classes = shape[:-1], shape[-1]
+    index_bytes = 4
+    if game is not None or position is not None:
+        if len(shape) != 3:
+            raise MuZeroError(f'with game and position, logits must be [unroll, batch, classes], got {tuple(shape)}')
+        if game is None or position is None:
+            raise MuZeroError('game and position: both or neither')
+        if targets.dim() != 3 or targets.shape[-1] != classes:
+            raise MuZeroError(f'targets must be [positions, games, {classes}], got {tuple(targets.shape)}')
+        for name, t in (('game', game), ('position', position)):
+            require_tensor(name, t, (torch.int32, torch.int64), device)
+            if t.shape != rows[1:]:
+                raise MuZeroError(f'{name} must have shape ({rows[1]},), got {tuple(t.shape)}')
+        if game.dtype != position.dtype:
+            raise MuZeroError(f'game is {game.dtype}, position {position.dtype}: both must be of one type')
+        index_bytes = 4 if game.dtype == torch.int32 else 8
+        game, position = game.contiguous(), position.contiguous()
+        positions, games = targets.shape[:2]
+    elif targets.shape != shape:
+        raise MuZeroError(f'targets have shape {tuple(targets.shape)}, logits {tuple(shape)}')
+    else:
+        positions, games = rows if len(rows) == 2 else (1, math.prod(rows))
+    wu = wb = 0
+    if weights is not None:
+        require_tensor('weights', weights, (torch.float32,), device)
+        if weights.requires_grad:
+            raise MuZeroError('the loss is not differentiable with respect to weights')
+        if weights.shape != rows:
             try:
-                weights = weights.expand(self.shape)
+                weights = weights.expand(rows)
             except RuntimeError:
-                raise MuZeroError(f'weights of shape {tuple(weights.shape)} do not broadcast to {tuple(self.shape)}') from None
-        require_hip(device)
-        cfg = self.cfg = _lib.Categorical()
-        classes = logits.shape[-1]
-        cfg.classes, cfg.dtype = classes, DTYPES[logits.dtype]
-        if len(self.shape) == 2:
-            cfg.unroll, cfg.batch = self.shape
-            if logits.stride(-1) != 1 and classes > 1:
-                logits = logits.contiguous()
-            cfg.logits_strides[0], cfg.logits_strides[1] = logits.stride(0), logits.stride(1)
-        else:
+                raise MuZeroError(f'weights of shape {tuple(weights.shape)} do not broadcast to {tuple(rows)}') from None
+        weights, wu, wb = _rows(weights)
+    require_hip(device)
+    if len(rows) == 2:
+        if logits.stride(-1) != 1 and classes > 1:
             logits = logits.contiguous()
-            cfg.unroll, cfg.batch = 1, math.prod(self.shape)
-            cfg.logits_strides[1] = classes
-        if indexed:
-            cfg.target_positions, cfg.target_games, cfg.index_bytes = targets.shape[0], targets.shape[1], game.element_size()
-            game, position = game.contiguous(), position.contiguous()
-        else:
-            cfg.target_positions, cfg.target_games = cfg.unroll, cfg.batch
-        weights = self._rows(weights, cfg.weight_strides) if weights is not None else None
-        self.tensors = logits, targets.contiguous(), game, position, weights
+        (unroll, batch), (zu, zb, _) = rows, logits.stride()
+    else:
+        logits = logits.contiguous()
+        unroll, batch, zu, zb = 1, math.prod(rows), 0, classes
+    config = _CONFIG.pack(unroll, batch, positions, games, classes, DTYPES[logits.dtype], index_bytes, 0, zu, zb, wu, wb)
+    return (logits, targets.contiguous(), game, position, weights), config
 
-    def _rows(self, t, strides):
-        """A tensor of the rows' shape as (u, b) strides."""
-        if len(self.shape) == 2:
-            strides[0], strides[1] = t.stride()
-            return t
-        t = t.contiguous()
-        strides[0], strides[1] = 0, 1
-        return t
 
-    def run(self, tensors, with_loss, with_grad, dloss=None):
-        ptr = lambda t: None if t is None else t.data_ptr()
-        logits = tensors[0]
-        loss = torch.empty(self.shape, dtype=torch.float32, device=self.device) if with_loss else None
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=self.device) if with_grad else None
-        if dloss is not None:
-            dloss = self._rows(dloss, self.cfg.dloss_strides)
-        launch(self.device, _lib.load().mz_categorical_loss, ctypes.byref(self.cfg), *[ptr(t) for t in tensors], ptr(dloss),
-               ptr(loss), ptr(grad))
-        return loss, grad
+def _run(tensors, config, with_loss, with_grad, dloss=None):
+    logits, targets, game, position, weights = tensors
+    shape, device = logits.shape, logits.device
+    gu = gb = 0
+    if dloss is not None:
+        dloss, gu, gb = _rows(dloss)
+    loss = torch.empty(shape[:-1], dtype=torch.float32, device=device) if with_loss else None
+    grad = torch.empty(shape, dtype=logits.dtype, device=device) if with_grad else None
+    launch(device, _lib.load().mz_categorical_loss, config + _DLOSS.pack(gu, gb), logits.data_ptr(), targets.data_ptr(), _ptr(game),
+           _ptr(position), _ptr(weights), _ptr(dloss), _ptr(loss), _ptr(grad))
+    return loss, grad
 
 
 class _CategoricalLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, call):
-        ctx.call = call
-        ctx.save_for_backward(*call.tensors)
-        loss, _ = call.run(call.tensors, True, False)
-        call.tensors = None              # what the backward pass needs, autograd keeps and frees
-        return loss
+    def forward(ctx, logits, tensors, config):
+        ctx.save_for_backward(*tensors)
+        ctx.config = config
+        return _run(tensors, config, True, False)[0]
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dloss):
-        return ctx.call.run(ctx.saved_tensors, False, True, dloss)[1], None
+        return _run(ctx.saved_tensors, ctx.config, False, True, dloss)[1], None, None
 
 
 def categorical_loss(logits: torch.Tensor, targets: torch.Tensor, game: Optional[torch.Tensor] = None,
@@ -119,11 +123,11 @@ def categorical_loss(logits: torch.Tensor, targets: torch.Tensor, game: Optional
     does not look at them).  weights broadcast over the rows; rows of weight 0 are not read and give 0 whatever they hold.  A
     class with target 0 adds nothing, also where its logit is -inf (an illegal move); a row whose logits are all -inf gives 0.
     A row of zero targets (past the end of a game) gives 0.  Differentiable once with respect to logits alone."""
-    call = _LossCall(logits, targets, game, position, weights)
+    tensors, config = _describe(logits, targets, game, position, weights)
     if not torch.is_grad_enabled() or not logits.requires_grad:
-        return call.run(call.tensors, True, False)[0]
-    refuse_capture_of_live_leaves(call.device, (logits,))
-    return remember_leaves(call.device, _CategoricalLoss.apply(logits, call))
+        return _run(tensors, config, True, False)[0]
+    refuse_capture_of_live_leaves(logits.device, (logits,))
+    return remember_leaves(logits.device, _CategoricalLoss.apply(logits, tensors, config))
 
 
 def categorical_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, game: Optional[torch.Tensor] = None,
@@ -132,8 +136,8 @@ def categorical_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, game:
     """-> (categorical_loss(...), the gradient of its sum with respect to logits, of their shape and type), in one launch
     and outside autograd: for a step whose factors are all in `weights` (importance of the samples, scale of the unrolled
     steps), which passes the gradient on with logits.backward(grad)."""
-    call = _LossCall(logits.detach() if isinstance(logits, torch.Tensor) else logits, targets, game, position, weights)
-    return call.run(call.tensors, True, True)
+    tensors, config = _describe(logits, targets, game, position, weights)
+    return _run(tensors, config, True, True)
 
 
 # ---- global norm and clipping --------------------------------------------------------------------------------------------
