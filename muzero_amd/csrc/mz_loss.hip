@@ -1,9 +1,15 @@
 // Cross entropy of unrolled logits against rows of the replay-target block, loss and gradient in one pass
 // (include/mzhip.h).
 //
-// Per row, in f32:  m = max z, s = sum exp(z - m), loss = w sum_{t != 0} t (m - z + log s),
-//                   dz = w (sum(t) exp(z - m) / s - t)
-// The target row is found by the sample's (position + step, game): no gathered copy of the targets exists.
+// Per row, in f32, with m = max z, s = sum exp(z - m), T = sum t:
+//   loss = w (sum over t != 0 of t (m - z) + T log s),   dz = w (T exp(z - m) / s - t)
+// (both terms of the loss are sums of what is not negative: nothing cancels).  The target row is found by the sample's
+// (position + step, game): no gathered copy of the targets exists.
+//
+// Bound by memory: logits and targets are read once, the gradient is written once.  A row belongs to W lanes (a power of
+// two), which hold all of it: up to K chunks of V adjacent classes each, read as one access a chunk, and two rounds of
+// shuffles: the maximum, then the three sums together.  A last chunk that would pass the row's end is moved back to end
+// with it; its first classes are its neighbour's too, which the sums leave out and the store writes a second time, alike.
 #include "mz_vec.h"
 #include <cmath>
 
@@ -11,13 +17,14 @@ namespace {
 
 using mz::bf16;
 using mz::f16;
+using mz::Vec;
 
 constexpr int kThreads = 256;
 constexpr int kMaxClasses = 4096;
 
 struct Loss {
     long U, B, P, G;
-    int C, wide;                        // wide: 8-byte indexes
+    int C, wide, lanes, chunks;         // wide: 8-byte indexes; lanes of a row, chunks of a row
     long zs[2], ws[2], gs[2];
     const void* z;
     const float *t, *w, *g;
@@ -30,51 +37,91 @@ __device__ inline long index_at(const void* p, int wide, long i) {
     return wide ? (long)static_cast<const int64_t*>(p)[i] : (long)static_cast<const int32_t*>(p)[i];
 }
 
-// one wavefront a row
-template <typename T>
+template <typename T, int V, int K>
 __global__ void __launch_bounds__(kThreads) categorical_kernel(Loss d) {
-    const int lane = threadIdx.x & 63;
-    const long rows = d.U * d.B, step = (long)gridDim.x * (kThreads / 64);
-    for (long row = blockIdx.x * (long)(kThreads / 64) + (threadIdx.x >> 6); row < rows; row += step) {
-        const long u = row / d.B, b = row - u * d.B;
-        const float w = d.w ? d.w[u * d.ws[0] + b * d.ws[1]] : 1.f;
-        const long position = d.position ? index_at(d.position, d.wide, b) : 0, game = d.game ? index_at(d.game, d.wide, b) : b;
-        const bool inside = position >= 0 && position < d.P - u && game >= 0 && game < d.G;
-        const T* z = static_cast<const T*>(d.z) + u * d.zs[0] + b * d.zs[1];
-        const float* t = d.t + (inside ? ((position + u) * d.G + game) * d.C : 0);
-        float m = -INFINITY, s = 0.f, l = 0.f, sum = 0.f;
-        bool nan = !inside;
-        if (w != 0.f && inside) {
-            for (int c = lane; c < d.C; c += 64) {
-                const float v = (float)z[c];
-                nan |= v != v;
-                m = fmaxf(m, v);
+    const int lane = threadIdx.x & (d.lanes - 1);
+    const long per_block = kThreads / d.lanes;
+    for (long u = blockIdx.y; u < d.U; u += gridDim.y)
+        for (long b = blockIdx.x * per_block + threadIdx.x / d.lanes; b < d.B; b += gridDim.x * per_block) {
+            const T* z = static_cast<const T*>(d.z) + u * d.zs[0] + b * d.zs[1];
+            const float w = d.w ? d.w[u * d.ws[0] + b * d.ws[1]] : 1.f;
+            const long position = d.position ? index_at(d.position, d.wide, b) : 0, game = d.game ? index_at(d.game, d.wide, b) : b;
+            const bool inside = position >= 0 && position < d.P - u && game >= 0 && game < d.G;
+            const float* t = d.t + (inside ? ((position + u) * d.G + game) * d.C : 0);
+            Vec<T, V> zv[K];
+            Vec<float, V> tv[K];
+            float e[K][V], m = -INFINITY, sums[3] = {0.f, 0.f, 0.f};
+            if (w != 0.f && inside) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks) {
+                        const int c = (lane + k * d.lanes) * V < d.C - V ? (lane + k * d.lanes) * V : d.C - V;
+                        zv[k] = mz::load<T, V>(z + c);
+                        tv[k] = mz::load<float, V>(t + c);
+                    }
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            e[k][i] = zv[k][i];
+                            m = fmaxf(m, e[k][i] != e[k][i] ? INFINITY : e[k][i]);      // a NaN ends in every sum
+                        }
             }
-            for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-            nan = __any(nan);
-        }
-        const bool empty = w == 0.f || (inside && !nan && m == -INFINITY);
-        float log_s = 0.f;
-        if (!empty && !nan) {
-            for (int c = lane; c < d.C; c += 64) s += __expf((float)z[c] - m);
-            s = mz::wave_sum(s);
-            log_s = logf(s);
-            for (int c = lane; c < d.C; c += 64) {
-                const float q = t[c];
-                sum += q;
-                if (q != 0.f) l = fmaf(q, (m - (float)z[c]) + log_s, l);
+            for (int k = d.lanes >> 1; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+            const bool empty = w == 0.f || (inside && m == -INFINITY), live = inside && !empty;
+            if (live)
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks) {
+                        const int twice = (lane + k * d.lanes) * V - (d.C - V);         // classes that the neighbour counts
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            const float below = m - e[k][i], q = tv[k][i];
+                            e[k][i] = __expf(-below);
+                            if (i >= twice) {
+                                sums[0] += e[k][i];
+                                sums[1] += q;
+                                if (q != 0.f) sums[2] = fmaf(q, below, sums[2]);
+                            }
+                        }
+                    }
+            for (int k = d.lanes >> 1; k; k >>= 1)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) sums[i] += __shfl_xor(sums[i], k);
+            const long row = u * d.B + b;
+            if (d.loss && lane == 0) d.loss[row] = empty ? 0.f : inside ? w * fmaf(sums[1], logf(sums[0]), sums[2]) : NAN;
+            if (d.grad) {
+                const float f = d.g ? w * d.g[u * d.gs[0] + b * d.gs[1]] : w, p = sums[1] / sums[0];
+                T* out = static_cast<T*>(d.grad) + row * d.C;
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks) {
+                        const int c = (lane + k * d.lanes) * V < d.C - V ? (lane + k * d.lanes) * V : d.C - V;
+                        float r[V];
+#pragma unroll
+                        for (int i = 0; i < V; ++i) r[i] = empty ? 0.f : inside ? f * fmaf(p, e[k][i], -tv[k][i]) : NAN;
+                        mz::store<T, V>(out + c, r);
+                    }
             }
-            l = mz::wave_sum(l);
-            sum = mz::wave_sum(sum);
         }
-        if (d.loss && lane == 0) d.loss[row] = empty ? 0.f : nan ? NAN : w * l;
-        if (d.grad) {
-            const float f = d.g ? w * d.g[u * d.gs[0] + b * d.gs[1]] : w, p = sum / s;
-            T* out = static_cast<T*>(d.grad) + row * d.C;
-            for (int c = lane; c < d.C; c += 64)
-                out[c] = (T)(empty ? 0.f : nan ? NAN : f * (p * __expf((float)z[c] - m) - t[c]));
-        }
-    }
+}
+
+template <typename T>
+void launch(Loss d, hipStream_t st) {
+    // four classes a chunk, two chunks a lane; more chunks only where a wavefront's lanes are used up
+    const int v = d.C >= 4 ? 4 : 1;
+    d.chunks = (d.C + v - 1) / v;
+    d.lanes = 1;
+    while (d.lanes < 64 && d.lanes * 2 < d.chunks) d.lanes <<= 1;
+    const int k = (d.chunks + d.lanes - 1) / d.lanes;
+    const long blocks = (d.B + kThreads / d.lanes - 1) / (kThreads / d.lanes);
+    const dim3 grid((unsigned)(blocks < 1L << 20 ? blocks : 1L << 20), (unsigned)(d.U < 65535 ? d.U : 65535));
+    if (v == 1) categorical_kernel<T, 1, 2><<<grid, kThreads, 0, st>>>(d);
+    else if (k <= 2) categorical_kernel<T, 4, 2><<<grid, kThreads, 0, st>>>(d);
+    else if (k <= 4) categorical_kernel<T, 4, 4><<<grid, kThreads, 0, st>>>(d);
+    else if (k <= 8) categorical_kernel<T, 4, 8><<<grid, kThreads, 0, st>>>(d);
+    else categorical_kernel<T, 4, 16><<<grid, kThreads, 0, st>>>(d);
 }
 
 }  // namespace
@@ -113,12 +160,17 @@ extern "C" int mz_categorical_loss(void* stream, const mz_categorical_t* c, cons
     d.position = position;
     d.loss = out_loss;
     d.grad = out_dlogits;
-    const long blocks = (d.U * d.B + kThreads / 64 - 1) / (kThreads / 64);
-    const unsigned grid = (unsigned)(blocks < (1L << 20) ? blocks : 1L << 20);
+    // rows that lie evenly behind one another, each with its own target row, are one long step
+    const auto even = [&](const long* stride) { return stride[0] == d.B * stride[1]; };
+    if (!game && !position && d.P == d.U && d.G == d.B && even(d.zs) && (!d.w || even(d.ws)) && (!d.g || even(d.gs))) {
+        d.B *= d.U;
+        d.G = d.B;
+        d.U = d.P = 1;
+    }
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (c->dtype == MZ_F32) categorical_kernel<float><<<grid, kThreads, 0, st>>>(d);
-    else if (c->dtype == MZ_F16) categorical_kernel<f16><<<grid, kThreads, 0, st>>>(d);
-    else categorical_kernel<bf16><<<grid, kThreads, 0, st>>>(d);
+    if (c->dtype == MZ_F32) launch<float>(d, st);
+    else if (c->dtype == MZ_F16) launch<f16>(d, st);
+    else launch<bf16>(d, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return mz::fail(MZ_ERR_HIP, "mz_categorical_loss launch failed: %s", hipGetErrorString(e));
     return MZ_OK;
