@@ -573,6 +573,22 @@ int mz_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* wo
                    float* out_norm);
 int mz_clip_by_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* const* outputs, double max_norm,
                            void* workspace, int64_t workspace_bytes, float* out_norm);
+/* The same for tensors that stay where they are from step to step: mz_tensor_table_build checks them once and writes
+ * n * MZ_TENSOR_TABLE_ENTRY bytes to host_table (HOST), which the caller copies to device memory and passes with
+ * out_table (HOST) to the other two.  The table may serve any number of calls and graphs at a time.  Tensors that
+ * overlap as above make a table for the norm alone (writable = 0, and mz_last_error() says which). */
+#define MZ_TENSOR_TABLE_ENTRY 32
+typedef struct mz_tensor_table {
+    int32_t entries, chunks;
+    int64_t chunk;
+    int32_t writable, reserved;
+} mz_tensor_table_t;
+int mz_tensor_table_build(int32_t n, const mz_tensor_t* tensors, void* const* outputs, void* host_table,
+                          mz_tensor_table_t* out_table);
+int mz_tensor_table_global_norm(void* stream, const mz_tensor_table_t* table, const void* device_table, void* workspace,
+                                int64_t workspace_bytes, float* out_norm);
+int mz_tensor_table_clip(void* stream, const mz_tensor_table_t* table, const void* device_table, double max_norm,
+                         void* workspace, int64_t workspace_bytes, float* out_norm);
 
 #ifdef __cplusplus
 }

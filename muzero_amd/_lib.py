@@ -74,10 +74,16 @@ class Tensor(ctypes.Structure):
     _fields_ = [('data', c_void_p), ('elements', c_int64), ('dtype', c_int32), ('reserved', c_int32)]
 
 
+class TensorTable(ctypes.Structure):
+    """mz_tensor_table_t"""
+    _fields_ = [('entries', c_int32), ('chunks', c_int32), ('chunk', c_int64), ('writable', c_int32), ('reserved', c_int32)]
+
+
 MZ_F32, MZ_F16, MZ_BF16 = 0, 1, 2
 MZ_ACT_NONE, MZ_ACT_RELU, MZ_ACT_SILU, MZ_ACT_GELU, MZ_ACT_TANH = 0, 1, 2, 3, 4
 MZ_GLOBAL_NORM_MAX_TENSORS = 8192
 MZ_GLOBAL_NORM_WORKSPACE = 32768
+MZ_TENSOR_TABLE_ENTRY = 32
 
 # name -> (restype, argtypes); every symbol include/mzhip.h declares
 PROTOTYPES = {
@@ -156,6 +162,9 @@ PROTOTYPES = {
     'mz_categorical_loss': (ctypes.c_int, [c_void_p, c_void_p] + [c_void_p] * 8),
     'mz_global_norm': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
     'mz_clip_by_global_norm': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_double, c_void_p, c_int64, c_void_p]),
+    'mz_tensor_table_build': (ctypes.c_int, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
+    'mz_tensor_table_global_norm': (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    'mz_tensor_table_clip': (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_int64, c_void_p]),
     'mz_env_cartpole_step': (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                             c_void_p, c_void_p]),
 }

@@ -1,13 +1,17 @@
 // Global norm of many tensors and clipping by it (include/mzhip.h).
 //
 //   norm = sqrt(sum g^2),  out = g * (max_norm / norm) where norm > max_norm, else g
-// The table of tensors travels in the kernel arguments (kBatch tensors a launch): nothing is uploaded, so a call may be
-// captured and takes other tensors the next time.  A tensor is cut into chunks; workgroups stride over the chunks of all
-// tensors.  Squares are summed in f64: exact squares of f32, no overflow, and one fixed order -- a workgroup leaves one
-// partial sum, and every workgroup of the next launch adds up all of them itself.
+//
+// Bound by memory: the norm reads every tensor once, clipping reads it again and writes it.  Tensors are cut into chunks of
+// one size, and workgroups stride over the chunks of all tensors.  Squares are summed in f64: exact squares of f32, no
+// overflow, and one fixed order -- a workgroup leaves one partial sum, and every workgroup of the second launch adds up all
+// of them itself, which takes less than a launch in between.  The table of tensors lies in device memory where the caller
+// keeps it (one launch a pass for any number of tensors); otherwise it travels in the kernel arguments, kBatch tensors a
+// launch, so that nothing is uploaded for tensors that are others in the next step.
 #include "mz_vec.h"
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <new>
 #include <vector>
 
@@ -18,50 +22,87 @@ using mz::f16;
 using mz::Vec;
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 128;                 // tensors a launch: 128 x 28 bytes of kernel arguments
-constexpr long kChunk = 16384;              // elements
-constexpr int64_t kMost = int64_t(1) << 43;  // elements: their chunks are counted in 32 bits
 constexpr int kPartials = MZ_GLOBAL_NORM_WORKSPACE / sizeof(double);
+constexpr int kBlocks = 2048;               // workgroups of a launch: eight a CU
+constexpr int64_t kMost = int64_t(1) << 43;  // elements: their chunks are counted in 32 bits
 
-struct Table {
-    const void* in[kBatch];
-    void* out[kBatch];
-    long elements[kBatch];
-    int first[kBatch];                      // chunk of all tensors that the tensor begins with
-    signed char dtype[kBatch];
-    int n, chunks;
+struct Entry {
+    const void* in;
+    void* out;
+    int64_t elements;
+    int32_t first;                          // chunk of all tensors that the tensor begins with
+    int32_t dtype;
 };
-static_assert(sizeof(Table) <= 3840, "the table has to fit the kernel arguments");
+static_assert(sizeof(Entry) == MZ_TENSOR_TABLE_ENTRY, "the header states an entry's size");
 
-__device__ inline int tensor_of(const Table& t, int chunk) {
-    int i = 0;
-    for (int k = 1; k < t.n; ++k) i = t.first[k] <= chunk ? k : i;      // later tensors begin at later chunks
-    return i;
+constexpr int kBatch = 112;                 // 3584 bytes of kernel arguments
+struct InArguments {
+    Entry e[kBatch];
+    int n, chunks;
+    long chunk;                             // elements of a chunk
+    __device__ const Entry* entries() const { return e; }
+};
+struct InMemory {
+    const Entry* e;
+    int n, chunks;
+    long chunk;
+    __device__ const Entry* entries() const { return e; }
+};
+
+// Index of the tensor that a chunk belongs to: the last that begins at or before it.  The wavefront's lanes look at 64 places
+// at once, so 112 tensors take two looks and 8192 three.
+__device__ inline int tensor_of(const Entry* e, int n, int chunk) {
+    int lo = 0, count = n;
+    while (count > 1) {
+        const int step = (count + 63) / 64, at = (int)(threadIdx.x & 63) * step;
+        const bool before = at < count && e[lo + at].first <= chunk;
+        const int last = __popcll(__ballot(before)) - 1;                   // the first place always counts
+        lo += last * step;
+        count = count - last * step < step ? count - last * step : step;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// f(element index, values) over n elements at p, U vectors a thread under way at once
+template <typename T, typename F, typename G>
+__device__ inline void walk(const T* p, long n, F vector, G single) {
+    constexpr int V = 16 / sizeof(T), U = 4;
+    const long whole = n / V;
+    for (long i = threadIdx.x; i < whole; i += U * kThreads) {
+        Vec<T, V> v[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (i + k * kThreads < whole) v[k] = mz::load<T, V>(p + (i + k * kThreads) * V);
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (i + k * kThreads < whole) vector((i + k * kThreads) * V, v[k]);
+    }
+    for (long i = whole * V + threadIdx.x; i < n; i += kThreads) single(i);
 }
 
 template <typename T>
-__device__ double squares(const T* p, long n) {
-    constexpr int V = 16 / sizeof(T);
+__device__ inline double squares(const T* p, long n) {
     double s = 0.0;
-    const long whole = n / V;
-    for (long i = threadIdx.x; i < whole; i += kThreads) {
-        const Vec<T, V> v = mz::load<T, V>(p + i * V);
+    walk(p, n,
+         [&](long, const Vec<T, 16 / sizeof(T)>& v) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) s = fma((double)v[k], (double)v[k], s);
-    }
-    for (long i = whole * V + threadIdx.x; i < n; i += kThreads) s = fma((double)(float)p[i], (double)(float)p[i], s);
+             for (int k = 0; k < (int)(16 / sizeof(T)); ++k) s = fma((double)v[k], (double)v[k], s);
+         },
+         [&](long i) { s = fma((double)(float)p[i], (double)(float)p[i], s); });
     return s;
 }
 
+template <typename Table>
 __global__ void __launch_bounds__(kThreads) norm_partials_kernel(Table t, double* partials) {
     __shared__ double scratch[kThreads / 64];
+    const Entry* e = t.entries();
     double s = 0.0;
     for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
-        const int i = tensor_of(t, chunk);
-        const long at = (chunk - t.first[i]) * kChunk, n = t.elements[i] - at < kChunk ? t.elements[i] - at : kChunk;
-        if (t.dtype[i] == MZ_F32) s += squares(static_cast<const float*>(t.in[i]) + at, n);
-        else if (t.dtype[i] == MZ_F16) s += squares(static_cast<const f16*>(t.in[i]) + at, n);
-        else s += squares(static_cast<const bf16*>(t.in[i]) + at, n);
+        const int i = tensor_of(e, t.n, chunk);
+        const long at = (chunk - e[i].first) * t.chunk, n = e[i].elements - at < t.chunk ? e[i].elements - at : t.chunk;
+        if (e[i].dtype == MZ_F32) s += squares(static_cast<const float*>(e[i].in) + at, n);
+        else if (e[i].dtype == MZ_F16) s += squares(static_cast<const f16*>(e[i].in) + at, n);
+        else s += squares(static_cast<const bf16*>(e[i].in) + at, n);
     }
     s = mz::block_sum<kThreads>(s, scratch);
     if (threadIdx.x == 0) partials[blockIdx.x] = s;
@@ -80,71 +121,56 @@ __global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double* par
 }
 
 template <typename T>
-__device__ void scale_chunk(const T* in, T* out, long n, float f) {
-    constexpr int V = 16 / sizeof(T);
-    const long whole = n / V;
-    for (long i = threadIdx.x; i < whole; i += kThreads) {
-        const Vec<T, V> v = mz::load<T, V>(in + i * V);
-        float r[V];
+__device__ inline void scale_chunk(const T* in, T* out, long n, float f) {
+    walk(in, n,
+         [&](long i, const Vec<T, 16 / sizeof(T)>& v) {
+             float r[16 / sizeof(T)];
 #pragma unroll
-        for (int k = 0; k < V; ++k) r[k] = v[k] * f;
-        mz::store<T, V>(out + i * V, r);
-    }
-    for (long i = whole * V + threadIdx.x; i < n; i += kThreads) out[i] = (T)((float)in[i] * f);
+             for (int k = 0; k < (int)(16 / sizeof(T)); ++k) r[k] = v[k] * f;
+             mz::store(out + i, r);
+         },
+         [&](long i) { out[i] = (T)((float)in[i] * f); });
 }
 
+// Chunks from the last to the first: what the norm read last is what the caches still hold.
+template <typename Table>
 __global__ void __launch_bounds__(kThreads) clip_kernel(Table t, const double* partials, int n, double max_norm, float* out_norm) {
     __shared__ double scratch[kThreads / 64];
+    const Entry* e = t.entries();
     const double norm = norm_of(partials, n, scratch);
     if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) *out_norm = (float)norm;
     const float f = norm <= max_norm ? 1.f : (float)(max_norm / norm);        // a NaN norm gives NaN
-    for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
-        const int i = tensor_of(t, chunk);
-        if (f == 1.f && t.in[i] == t.out[i]) continue;                        // nothing to change in place
-        const long at = (chunk - t.first[i]) * kChunk, m = t.elements[i] - at < kChunk ? t.elements[i] - at : kChunk;
-        if (t.dtype[i] == MZ_F32) scale_chunk(static_cast<const float*>(t.in[i]) + at, static_cast<float*>(t.out[i]) + at, m, f);
-        else if (t.dtype[i] == MZ_F16) scale_chunk(static_cast<const f16*>(t.in[i]) + at, static_cast<f16*>(t.out[i]) + at, m, f);
-        else scale_chunk(static_cast<const bf16*>(t.in[i]) + at, static_cast<bf16*>(t.out[i]) + at, m, f);
+    for (int chunk = t.chunks - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
+        const int i = tensor_of(e, t.n, chunk);
+        if (f == 1.f && e[i].in == e[i].out) continue;                        // nothing to change in place
+        const long at = (chunk - e[i].first) * t.chunk, m = e[i].elements - at < t.chunk ? e[i].elements - at : t.chunk;
+        if (e[i].dtype == MZ_F32) scale_chunk(static_cast<const float*>(e[i].in) + at, static_cast<float*>(e[i].out) + at, m, f);
+        else if (e[i].dtype == MZ_F16) scale_chunk(static_cast<const f16*>(e[i].in) + at, static_cast<f16*>(e[i].out) + at, m, f);
+        else scale_chunk(static_cast<const bf16*>(e[i].in) + at, static_cast<bf16*>(e[i].out) + at, m, f);
     }
 }
 
-// Calls f(table, grid) for every launch's part of the tensors; empty tensors are left out.
-template <typename F>
-void for_each_table(int32_t n, const mz_tensor_t* tensors, void* const* outputs, F f) {
-    Table t;
-    t.n = t.chunks = 0;
-    const int launches = (n + kBatch - 1) / kBatch;            // their workgroups share the room for partial sums
-    const int most = kPartials / launches < 2048 ? kPartials / launches : 2048;
-    for (int32_t i = 0; i < n; ++i) {
-        if (!tensors[i].elements) continue;
-        t.in[t.n] = tensors[i].data;
-        t.out[t.n] = outputs ? outputs[i] : tensors[i].data;
-        t.elements[t.n] = tensors[i].elements;
-        t.first[t.n] = t.chunks;
-        t.dtype[t.n] = (signed char)tensors[i].dtype;
-        t.chunks += (int)((tensors[i].elements + kChunk - 1) / kChunk);
-        if (++t.n == kBatch) {
-            f(t, t.chunks < most ? t.chunks : most);
-            t.n = t.chunks = 0;
-        }
-    }
-    if (t.n) f(t, t.chunks < most ? t.chunks : most);
-}
+// ---- host -------------------------------------------------------------------------------------------------------------
 
-int check(int32_t n, const mz_tensor_t* tensors, void* workspace, int64_t bytes) {
+int check(int32_t n, const mz_tensor_t* tensors, int64_t* total) {
     MZ_REQUIRE(n >= 1 && n <= MZ_GLOBAL_NORM_MAX_TENSORS, "between 1 and %d tensors, got %d", MZ_GLOBAL_NORM_MAX_TENSORS, n);
     MZ_REQUIRE(tensors, "tensors is NULL");
-    MZ_REQUIRE(workspace && bytes >= MZ_GLOBAL_NORM_WORKSPACE, "workspace of %lld bytes, %d needed", (long long)bytes, MZ_GLOBAL_NORM_WORKSPACE);
-    int64_t total = 0;
+    *total = 0;
     for (int32_t i = 0; i < n; ++i) {
         const int item = mz::dtype_size(tensors[i].dtype);
         MZ_REQUIRE(item, "tensor %d: dtype %d is not one of mz_dtype", i, tensors[i].dtype);
-        MZ_REQUIRE(tensors[i].elements >= 0 && tensors[i].elements <= kMost - total, "tensor %d: %lld elements (2^43 in all at most)", i,
+        MZ_REQUIRE(tensors[i].elements >= 0 && tensors[i].elements <= kMost - *total, "tensor %d: %lld elements (2^43 in all at most)", i,
                    (long long)tensors[i].elements);
-        total += tensors[i].elements;
         MZ_REQUIRE(tensors[i].data || !tensors[i].elements, "tensor %d: data is NULL", i);
         MZ_REQUIRE((uintptr_t)tensors[i].data % item == 0, "tensor %d: data is not aligned to its type", i);
+        *total += tensors[i].elements;
     }
+    return MZ_OK;
+}
+
+int check_workspace(void* workspace, int64_t bytes, const float* out_norm) {
+    MZ_REQUIRE(workspace && bytes >= MZ_GLOBAL_NORM_WORKSPACE, "workspace of %lld bytes, %d needed", (long long)bytes, MZ_GLOBAL_NORM_WORKSPACE);
+    MZ_REQUIRE(out_norm, "out_norm is NULL");
     return MZ_OK;
 }
 
@@ -179,58 +205,155 @@ int check_overlap(int32_t n, const mz_tensor_t* tensors, void* const* outputs) {
     return MZ_OK;
 }
 
+int check_written(int32_t n, const mz_tensor_t* tensors, void* const* outputs) {
+    try {
+        return check_overlap(n, tensors, outputs);
+    } catch (const std::bad_alloc&) {
+        return mz::fail(MZ_ERR_OOM, "no host memory for the overlap check");
+    }
+}
+
+// A chunk for each of a launch's workgroups while a chunk still is eight vectors a thread, up to 64 K elements.
+long chunk_of(int64_t total) {
+    long c = 2048;
+    while (c < 65536 && c * kBlocks < total) c <<= 1;
+    return c;
+}
+
+Entry entry_of(const mz_tensor_t& t, void* out, int32_t first) { return {t.data, out, t.elements, first, t.dtype}; }
+int chunks_of(int64_t elements, long chunk) { return (int)((elements + chunk - 1) / chunk); }
+
+// Calls f(table, workgroups) for every launch's part of the tensors; empty tensors are left out.
+template <typename F>
+void for_each_table(int32_t n, const mz_tensor_t* tensors, void* const* outputs, int64_t total, F f) {
+    InArguments t;
+    t.n = t.chunks = 0;
+    t.chunk = chunk_of(total);
+    const int launches = (n + kBatch - 1) / kBatch;            // their workgroups share the room for partial sums
+    const int most = kPartials / launches < kBlocks ? kPartials / launches : kBlocks;
+    for (int32_t i = 0; i < n; ++i) {
+        if (!tensors[i].elements) continue;
+        t.e[t.n] = entry_of(tensors[i], outputs ? outputs[i] : tensors[i].data, t.chunks);
+        t.chunks += chunks_of(tensors[i].elements, t.chunk);
+        if (++t.n == kBatch) {
+            f(t, t.chunks < most ? t.chunks : most);
+            t.n = t.chunks = 0;
+        }
+    }
+    if (t.n) f(t, t.chunks < most ? t.chunks : most);
+}
+
 int launched(const char* what) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return mz::fail(MZ_ERR_HIP, "%s launch failed: %s", what, hipGetErrorString(e));
     return MZ_OK;
 }
 
-int partials_of(hipStream_t st, int32_t n, const mz_tensor_t* tensors, double* partials) {
+int partials_of(hipStream_t st, int32_t n, const mz_tensor_t* tensors, int64_t total, double* partials) {
     int used = 0;
-    for_each_table(n, tensors, nullptr, [&](const Table& t, int grid) {
+    for_each_table(n, tensors, nullptr, total, [&](const InArguments& t, int grid) {
         norm_partials_kernel<<<grid, kThreads, 0, st>>>(t, partials + used);
         used += grid;
     });
     return used;
 }
 
+int check_table(const mz_tensor_table_t* t, const void* device_table) {
+    MZ_REQUIRE(t, "table is NULL");
+    MZ_REQUIRE(t->entries >= 0 && t->entries <= MZ_GLOBAL_NORM_MAX_TENSORS && t->chunks >= t->entries && t->chunk >= 1, "not a table of mz_tensor_table_build");
+    MZ_REQUIRE(device_table || !t->entries, "device_table is NULL");
+    return MZ_OK;
+}
+InMemory in_memory(const mz_tensor_table_t* t, const void* device_table) {
+    return {static_cast<const Entry*>(device_table), t->entries, t->chunks, t->chunk};
+}
+int blocks_of(const mz_tensor_table_t* t) { return t->chunks < kBlocks ? t->chunks : kBlocks; }
+
 }  // namespace
 
 extern "C" {
 
 int mz_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* workspace, int64_t workspace_bytes, float* out_norm) {
-    const int bad = check(n, tensors, workspace, workspace_bytes);
+    int64_t total;
+    int bad = check(n, tensors, &total);
+    if (!bad) bad = check_workspace(workspace, workspace_bytes, out_norm);
     if (bad) return bad;
-    MZ_REQUIRE(out_norm, "out_norm is NULL");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     double* partials = static_cast<double*>(workspace);
-    const int used = partials_of(st, n, tensors, partials);
+    const int used = partials_of(st, n, tensors, total, partials);
     norm_finish_kernel<<<1, kThreads, 0, st>>>(partials, used, out_norm);
     return launched("mz_global_norm");
 }
 
 int mz_clip_by_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* const* outputs, double max_norm,
                            void* workspace, int64_t workspace_bytes, float* out_norm) {
-    int bad = check(n, tensors, workspace, workspace_bytes);
+    int64_t total;
+    int bad = check(n, tensors, &total);
+    if (!bad) bad = check_workspace(workspace, workspace_bytes, out_norm);
+    if (!bad) bad = check_written(n, tensors, outputs);
     if (bad) return bad;
-    MZ_REQUIRE(out_norm, "out_norm is NULL");
     MZ_REQUIRE(max_norm >= 0, "max_norm must be >= 0");
-    try {
-        bad = check_overlap(n, tensors, outputs);
-    } catch (const std::bad_alloc&) {
-        return mz::fail(MZ_ERR_OOM, "no host memory for the overlap check");
-    }
-    if (bad) return bad;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     double* partials = static_cast<double*>(workspace);
-    const int used = partials_of(st, n, tensors, partials);
+    const int used = partials_of(st, n, tensors, total, partials);
     float* out = out_norm;
-    for_each_table(n, tensors, outputs, [&](const Table& t, int grid) {
+    for_each_table(n, tensors, outputs, total, [&](const InArguments& t, int grid) {
         clip_kernel<<<grid, kThreads, 0, st>>>(t, partials, used, max_norm, out);
         out = nullptr;
     });
     if (out) norm_finish_kernel<<<1, kThreads, 0, st>>>(partials, used, out);      // empty tensors only
     return launched("mz_clip_by_global_norm");
+}
+
+int mz_tensor_table_build(int32_t n, const mz_tensor_t* tensors, void* const* outputs, void* host_table, mz_tensor_table_t* out_table) {
+    int64_t total;
+    const int bad = check(n, tensors, &total);
+    if (bad) return bad;
+    MZ_REQUIRE(host_table && out_table, "host_table/out_table is NULL");
+    Entry* e = static_cast<Entry*>(host_table);
+    mz_tensor_table_t t = {};
+    t.chunk = chunk_of(total);
+    // a table that clipping may not write still serves the norm
+    t.writable = check_written(n, tensors, outputs) == MZ_OK;
+    for (int32_t i = 0; i < n; ++i) {
+        if (!tensors[i].elements) continue;
+        e[t.entries++] = entry_of(tensors[i], outputs ? outputs[i] : tensors[i].data, t.chunks);
+        t.chunks += chunks_of(tensors[i].elements, t.chunk);
+    }
+    *out_table = t;
+    return MZ_OK;
+}
+
+int mz_tensor_table_global_norm(void* stream, const mz_tensor_table_t* table, const void* device_table, void* workspace,
+                                int64_t workspace_bytes, float* out_norm) {
+    int bad = check_table(table, device_table);
+    if (!bad) bad = check_workspace(workspace, workspace_bytes, out_norm);
+    if (bad) return bad;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    double* partials = static_cast<double*>(workspace);
+    const int blocks = blocks_of(table);
+    if (blocks) norm_partials_kernel<<<blocks, kThreads, 0, st>>>(in_memory(table, device_table), partials);
+    norm_finish_kernel<<<1, kThreads, 0, st>>>(partials, blocks, out_norm);
+    return launched("mz_tensor_table_global_norm");
+}
+
+int mz_tensor_table_clip(void* stream, const mz_tensor_table_t* table, const void* device_table, double max_norm, void* workspace,
+                         int64_t workspace_bytes, float* out_norm) {
+    int bad = check_table(table, device_table);
+    if (!bad) bad = check_workspace(workspace, workspace_bytes, out_norm);
+    if (bad) return bad;
+    MZ_REQUIRE(table->writable, "tensors of the table overlap: they cannot be written");
+    MZ_REQUIRE(max_norm >= 0, "max_norm must be >= 0");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    double* partials = static_cast<double*>(workspace);
+    const int blocks = blocks_of(table);
+    if (!blocks) {
+        norm_finish_kernel<<<1, kThreads, 0, st>>>(partials, 0, out_norm);
+    } else {
+        norm_partials_kernel<<<blocks, kThreads, 0, st>>>(in_memory(table, device_table), partials);
+        clip_kernel<<<blocks, kThreads, 0, st>>>(in_memory(table, device_table), partials, blocks, max_norm, out_norm);
+    }
+    return launched("mz_tensor_table_clip");
 }
 
 }  // extern "C"

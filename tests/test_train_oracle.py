@@ -176,3 +176,25 @@ def test_clip_refuses_overlap_before_any_launch():
                dict(tensors=[(A, 1 << 42, 0), (A + (1 << 44), 1 << 42, 0), (A + (1 << 45), 1, 0)])]
     for kw in refused:
         assert clip(**kw) == -1, kw
+
+
+def test_tensor_tables_are_checked_where_they_are_built():
+    L, lib = _lib()
+    A = 0x100000
+    build = lambda table, n, host, out: lib.mz_tensor_table_build(n, (L.Tensor * len(table))(*table), None, host, ctypes.byref(out) if out else None)
+    two = [L.Tensor(data=A, elements=5000, dtype=0), L.Tensor(data=A + (1 << 20), elements=0, dtype=1), L.Tensor(data=A + (1 << 20), elements=1, dtype=2)]
+    host, info = (ctypes.c_char * (3 * L.MZ_TENSOR_TABLE_ENTRY))(), L.TensorTable()
+    assert build(two, 3, host, info) == 0
+    assert (info.entries, info.writable) == (2, 1) and info.chunks == -(-5000 // info.chunk) + 1       # empty tensors are left out
+    assert build(two, 3, None, info) == -1 and build(two, 0, host, info) == -1
+    assert build([L.Tensor(data=None, elements=1, dtype=0)], 1, host, info) == -1
+    assert build([two[0], two[0]], 2, host, info) == 0 and info.writable == 0
+    args = (0x100, L.MZ_GLOBAL_NORM_WORKSPACE, 0x100)
+    assert lib.mz_tensor_table_clip(None, ctypes.byref(info), 0x100, 1.0, *args) == -1                  # overlapping tensors
+    assert build(two, 3, host, info) == 0
+    assert lib.mz_tensor_table_clip(None, ctypes.byref(info), 0x100, -1.0, *args) == -1
+    assert lib.mz_tensor_table_clip(None, ctypes.byref(info), None, 1.0, *args) == -1
+    assert lib.mz_tensor_table_clip(None, ctypes.byref(L.TensorTable(entries=-1)), 0x100, 1.0, *args) == -1
+    assert lib.mz_tensor_table_global_norm(None, None, 0x100, *args) == -1
+    assert lib.mz_tensor_table_global_norm(None, ctypes.byref(info), 0x100, 0x100, L.MZ_GLOBAL_NORM_WORKSPACE - 1, 0x100) == -1
+    assert lib.mz_tensor_table_global_norm(None, ctypes.byref(info), 0x100, 0x100, L.MZ_GLOBAL_NORM_WORKSPACE, None) == -1

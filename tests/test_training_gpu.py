@@ -423,3 +423,64 @@ def test_a_training_step_on_replay_targets():
     total = clip_by_global_norm(grads, 0.5, out=out)
     check_clip(grads, 0.5, out, total)
     assert abs(float(torch.linalg.vector_norm(flat.double())) - 0.5) < 1e-6
+
+
+@pytest.mark.parametrize('n', [1, 63, 64, 65, 111, 112, 113, 700, 4097, 8192])
+def test_clip_of_many_tensors_kept_and_by_the_call(n):
+    from muzero_amd.training import GradientSet, clip_by_global_norm
+    gen = torch.Generator(device='cuda').manual_seed(n)
+    pool = torch.randn(n * 40, generator=gen, device='cuda')
+    sizes = [1 + (7 * i) % 40 for i in range(n)]
+    tensors = [pool[40 * i:40 * i + k] for i, k in enumerate(sizes)]
+    kept, called = [torch.full_like(t, 9) for t in tensors], torch.full_like(pool, 9)
+    norm = GradientSet(tensors, kept).clip_by_global_norm(1.0)
+    other = clip_by_global_norm(tensors, 1.0, out=[called[40 * i:40 * i + k] for i, k in enumerate(sizes)])
+    whole = torch.cat(tensors)
+    check_clip([whole], 1.0, [torch.cat(kept)], norm)
+    # the two take their partial sums in other orders: 64-bit sums rounded to 32 bits, at most one step apart
+    assert abs(float(norm) - float(other)) <= 2 * to.U32 * float(norm)
+    check_clip([whole], 1.0, [torch.cat([called[40 * i:40 * i + k] for i, k in enumerate(sizes)])], other)
+    gaps = torch.ones(n, 40, dtype=torch.bool, device='cuda')
+    for i, k in enumerate(sizes):
+        gaps[i, :k] = False
+    assert (called[gaps.ravel()] == 9).all()
+
+
+def test_a_set_on_several_streams_and_in_two_graphs_at_once():
+    from muzero_amd.training import GradientSet
+    tensors = tensors_of([1 << 20, 77, 4096], (F32,))
+    out = [torch.empty_like(t) for t in tensors]
+    kept = GradientSet(tensors, out)
+    want = kept.clip_by_global_norm(0.5)
+    torch.cuda.synchronize()
+    first = [o.clone() for o in out]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    norms = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            norms += [kept.global_norm() for _ in range(5)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    captured = []
+    torch.cuda.synchronize()
+    for g in graphs:
+        with torch.cuda.graph(g):
+            captured.append(kept.clip_by_global_norm(0.5))
+    for o in out:
+        o.zero_()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want) for v in norms + captured) and all(torch.equal(a, b) for a, b in zip(out, first))
+
+
+def test_a_set_is_not_made_inside_a_capture():
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.training import GradientSet
+    t = torch.ones(4, device='cuda')
+    with pytest.raises(MuZeroError, match='capture'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            GradientSet([t])
