@@ -125,17 +125,25 @@ __device__ inline void column_sum(float (&v)[V], const Norm& d, float* scratch) 
             for (int k = 0; k < V; ++k) v[k] += scratch[k * TH + (w << 6) + t];
 }
 
-template <typename T>
-__device__ inline float param(const void* p, int f32, int c) {
-    return f32 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
+template <typename T, int V>
+__device__ inline void load_param(const void* p, int f32, int c, float missing, float (&v)[V]) {
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = missing;
+    } else if (f32) {
+        const Vec<float, V> r = mz::load<float, V>(static_cast<const float*>(p) + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = r[i];
+    } else {
+        const Vec<T, V> r = mz::load<T, V>(static_cast<const T*>(p) + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = r[i];
+    }
 }
 template <typename T, int V>
 __device__ inline void load_params(const Norm& d, int c, float (&w)[V], float (&b)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        w[i] = d.w ? param<T>(d.w, d.params_f32, c + i) : 1.f;
-        b[i] = d.b ? param<T>(d.b, d.params_f32, c + i) : 0.f;
-    }
+    load_param<T, V>(d.w, d.params_f32, c, 1.f, w);
+    load_param<T, V>(d.b, d.params_f32, c, 0.f, b);
 }
 
 // No activation and relu share their code: a floor below which z is cut, and a threshold that z has to be above for its slope.
@@ -145,27 +153,48 @@ struct Cut {
     __device__ float operator()(float z) const { return z < floor ? floor : z; }              // a NaN stays
     __device__ float slope(float z) const { return z <= edge ? 0.f : 1.f; }
 };
+// The others from one exponential and one reciprocal, each within a step or two of f32 (v_exp_f32, v_rcp_f32): with the
+// library's exact division, erf and tanh the arithmetic took longer than the memory.
+__device__ inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950409f); }
+__device__ inline float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
 struct Silu {
     __device__ explicit Silu(int) {}
-    __device__ float operator()(float z) const { return z / (1.f + __expf(-z)); }
+    __device__ static float sigmoid(float z) { return fast_rcp(1.f + fast_exp(-z)); }
+    __device__ float operator()(float z) const { return z * sigmoid(z); }
     __device__ float slope(float z) const {
-        const float s = 1.f / (1.f + __expf(-z));
+        const float s = sigmoid(z);
         return s * fmaf(z, 1.f - s, 1.f);
     }
 };
+// z times the normal distribution's integral, by the five-term approximation of Abramowitz and Stegun 7.1.26 (off by at most
+// 1.5e-7 / 2 everywhere, relatively good in the lower tail, where it is taken as it stands), with the exponential that the
+// density needs too.
 struct Gelu {
     __device__ explicit Gelu(int) {}
-    __device__ float operator()(float z) const { return 0.5f * z * (1.f + erff(z * 0.70710678f)); }
+    __device__ static float below(float z, float e) {          // e = exp(-z^2 / 2)
+        const float t = fast_rcp(fmaf(fabsf(z), 0.3275911f * 0.70710678f, 1.f));
+        const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
+                                         0.5f * -0.284496736f), 0.5f * 0.254829592f);
+        return z < 0.f ? p * e : fmaf(-p, e, 1.f);
+    }
+    __device__ float operator()(float z) const { return z * below(z, fast_exp(-0.5f * z * z)); }
     __device__ float slope(float z) const {
-        return fmaf(z * 0.39894228f, __expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678f)));
+        const float e = fast_exp(-0.5f * z * z);
+        return fmaf(z * 0.39894228f, e, below(z, e));
     }
 };
+// (1 - q) / (1 + q) with q = exp(-2 |z|); where 1 - q cancels, the first terms of the series of tanh
 struct Tanh {
     __device__ explicit Tanh(int) {}
-    __device__ float operator()(float z) const { return tanhf(z); }
+    __device__ float operator()(float z) const {
+        const float q = fast_exp(-2.f * fabsf(z)), y = z * z;
+        const float near = z * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+        return y < 0.0625f ? near : copysignf((1.f - q) * fast_rcp(1.f + q), z);
+    }
     __device__ float slope(float z) const {
-        const float t = tanhf(z);
-        return fmaf(-t, t, 1.f);
+        const float q = fast_exp(-2.f * fabsf(z)), r = fast_rcp(1.f + q);
+        return 4.f * q * r * r;
     }
 };
 template <typename F>
@@ -252,10 +281,9 @@ __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
     __shared__ float scratch[2][TH];
     const int S = (int)d.S, step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
-    const long units = (d.N + d.samples - 1) / d.samples * d.tiles;
-    for (long unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        const long set = unit / d.tiles, n0 = set * d.samples;
-        const Lane l = lane_of<V>(d, (int)(unit - set * d.tiles));
+    for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y)
+    for (long n0 = (long)blockIdx.x * d.samples; n0 < d.N; n0 += (long)gridDim.x * d.samples) {
+        const Lane l = lane_of<V>(d, tile);
         const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;       // samples of this workgroup
         const bool live = l.live && l.sample < left;
         const int j = live ? l.sample : 0;
@@ -309,11 +337,12 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
     __shared__ float scratch[TH == 64 ? 1 : TH * (V > 2 ? 2 * V : 4)];
     const int S = (int)d.S, step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
-    const long block = blockIdx.x / d.tiles;
-    const Lane l = lane_of<V>(d, (int)(blockIdx.x - block * d.tiles));
+    const long block = blockIdx.x;
+    int turn = 0;
+    for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y) {
+    const Lane l = lane_of<V>(d, tile);
     float w[V], b[V], s1[V] = {}, s2[V] = {};
     load_params<T, V>(d, l.ch, w, b);
-    int turn = 0;
     for (long n0 = block * d.samples; n0 < d.N; n0 += d.blocks * d.samples, turn ^= 1) {
         const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;
         const bool live = l.live && l.sample < left;
@@ -356,16 +385,14 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
             }
         });
     }
-    if (!d.dw && !d.db) return;
+    if (!d.dw && !d.db) continue;
     column_sum<TH>(s1, d, scratch);
     column_sum<TH>(s2, d, TH == 64 ? scratch : scratch + TH * V);
+    if (TH > 64) __syncthreads();                           // before another tile's sums
     if (l.live && l.row == 0 && l.sample == 0) {
-        float* ws = d.ws + block * 2 * d.C + l.ch;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            ws[i] = s1[i];
-            ws[d.C + i] = s2[i];
-        }
+        mz::store<float, V>(d.ws + block * 2 * d.C + l.ch, s1);
+        mz::store<float, V>(d.ws + block * 2 * d.C + d.C + l.ch, s2);
+    }
     }
 }
 
@@ -554,11 +581,8 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
         column_sum<kSplitThreads>(s2, d, scratch[0]);
         if (l.live && l.row == 0) {
             float* ws = d.ws + (p.n * d.splits + p.split) * 2 * d.C + l.ch;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                ws[i] = s1[i];
-                ws[d.C + i] = s2[i];
-            }
+            mz::store<float, V>(ws, s1);
+            mz::store<float, V>(ws + d.C, s2);
             if (l.vec == 0) {
                 float* at = d.ws + d.N * d.splits * 2 * d.C + 2 * part_at(d, p, l);
                 at[0] = aq[0];
@@ -676,7 +700,7 @@ void forward(const Plan& p, int v, hipStream_t st) {
     with_vector<T>(v, [&](auto v_) {
         constexpr int V = v_.value;
         if (p.k) {
-            const unsigned grid = grid_of((d.N + d.samples - 1) / d.samples * d.tiles);
+            const dim3 grid(grid_of((d.N + d.samples - 1) / d.samples), d.tiles < 65535 ? d.tiles : 65535);
             with_size(p, [&](auto th, auto k) { norm_forward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
         } else {
             const unsigned grid = grid_of(d.N * d.tiles * d.splits);
@@ -694,7 +718,7 @@ void backward(const Plan& p, int v, hipStream_t st) {
         with_vector<T>(v, [&](auto v_) {
             constexpr int V = v_.value;
             if (p.k) {
-                const unsigned grid = (unsigned)(d.blocks * d.tiles);
+                const dim3 grid((unsigned)d.blocks, d.tiles < 65535 ? d.tiles : 65535);
                 with_size(p, [&](auto th, auto k) { norm_backward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
             } else {
                 const unsigned grid = grid_of(d.N * d.tiles * d.splits);
