@@ -282,52 +282,52 @@ __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
     const int S = (int)d.S, step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
     for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y)
-    for (long n0 = (long)blockIdx.x * d.samples; n0 < d.N; n0 += (long)gridDim.x * d.samples) {
-        const Lane l = lane_of<V>(d, tile);
-        const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;       // samples of this workgroup
-        const bool live = l.live && l.sample < left;
-        const int j = live ? l.sample : 0;
-        Vec<T, V> xv[K], rv[K];
-        load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
-        if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
-        float w[V], b[V];
-        load_params<T, V>(d, l.ch, w, b);
-        float sum[1] = {0.f};
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (k * step < S) {
-                float p = 0.f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) p += xv[k][i];
-                sum[0] += live && l.row + k * step < S ? p : 0.f;
-            }
-        group_sum<TH>(sum, d, scratch[0]);
-        const float mu = sum[0] * inv;
-        sum[0] = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (k * step < S) {
-                float p = 0.f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) p = fmaf(xv[k][i] - mu, xv[k][i] - mu, p);
-                sum[0] += live && l.row + k * step < S ? p : 0.f;
-            }
-        group_sum<TH>(sum, d, scratch[1]);
-        const float rs = 1.f / sqrtf(sum[0] * inv + d.eps);
-        if (!live) continue;
-        if (d.mean && l.vec == 0 && l.row == 0) {
-            d.mean[(n0 + j) * d.G + l.g] = mu;
-            d.rstd[(n0 + j) * d.G + l.g] = rs;
-        }
-        T* y = static_cast<T*>(d.y) + n0 * d.S * d.C;
-        const int at = (j * S + l.row) * d.C + l.ch;
-        with_activation(d.act, [&](auto act) {
+        for (long n0 = (long)blockIdx.x * d.samples; n0 < d.N; n0 += (long)gridDim.x * d.samples) {
+            const Lane l = lane_of<V>(d, tile);
+            const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;       // samples of this workgroup
+            const bool live = l.live && l.sample < left;
+            const int j = live ? l.sample : 0;
+            Vec<T, V> xv[K], rv[K];
+            load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
+            if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
+            float w[V], b[V];
+            load_params<T, V>(d, l.ch, w, b);
+            float sum[1] = {0.f};
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (l.row + k * step < S)
-                    apply<T, V>(xv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, y + (unsigned)(at + k * step * d.C));
-        });
-    }
+                if (k * step < S) {
+                    float p = 0.f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) p += xv[k][i];
+                    sum[0] += live && l.row + k * step < S ? p : 0.f;
+                }
+            group_sum<TH>(sum, d, scratch[0]);
+            const float mu = sum[0] * inv;
+            sum[0] = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k * step < S) {
+                    float p = 0.f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) p = fmaf(xv[k][i] - mu, xv[k][i] - mu, p);
+                    sum[0] += live && l.row + k * step < S ? p : 0.f;
+                }
+            group_sum<TH>(sum, d, scratch[1]);
+            const float rs = 1.f / sqrtf(sum[0] * inv + d.eps);
+            if (!live) continue;
+            if (d.mean && l.vec == 0 && l.row == 0) {
+                d.mean[(n0 + j) * d.G + l.g] = mu;
+                d.rstd[(n0 + j) * d.G + l.g] = rs;
+            }
+            T* y = static_cast<T*>(d.y) + n0 * d.S * d.C;
+            const int at = (j * S + l.row) * d.C + l.ch;
+            with_activation(d.act, [&](auto act) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (l.row + k * step < S)
+                        apply<T, V>(xv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, y + (unsigned)(at + k * step * d.C));
+            });
+        }
 }
 
 // A workgroup keeps its tile and strides over the samples: the channels' sums for dweight and dbias stay in registers and
@@ -340,59 +340,59 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
     const long block = blockIdx.x;
     int turn = 0;
     for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y) {
-    const Lane l = lane_of<V>(d, tile);
-    float w[V], b[V], s1[V] = {}, s2[V] = {};
-    load_params<T, V>(d, l.ch, w, b);
-    for (long n0 = block * d.samples; n0 < d.N; n0 += d.blocks * d.samples, turn ^= 1) {
-        const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;
-        const bool live = l.live && l.sample < left;
-        const int j = live ? l.sample : 0;
-        Vec<T, V> xv[K], gv[K], rv[K];
-        load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
-        load_rows<T, V, K>(gv, static_cast<const T*>(d.dy) + n0 * d.ds[0], j * (int)d.ds[0] + l.ch, (int)d.ds[1], l.row, step, S);
-        if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
-        const float mu = d.mean[(n0 + j) * d.G + l.g], rs = d.rstd[(n0 + j) * d.G + l.g];
-        float aq[2] = {0.f, 0.f};
-        with_activation(d.act, [&](auto act) {
+        const Lane l = lane_of<V>(d, tile);
+        float w[V], b[V], s1[V] = {}, s2[V] = {};
+        load_params<T, V>(d, l.ch, w, b);
+        for (long n0 = block * d.samples; n0 < d.N; n0 += d.blocks * d.samples, turn ^= 1) {
+            const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;
+            const bool live = l.live && l.sample < left;
+            const int j = live ? l.sample : 0;
+            Vec<T, V> xv[K], gv[K], rv[K];
+            load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
+            load_rows<T, V, K>(gv, static_cast<const T*>(d.dy) + n0 * d.ds[0], j * (int)d.ds[0] + l.ch, (int)d.ds[1], l.row, step, S);
+            if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
+            const float mu = d.mean[(n0 + j) * d.G + l.g], rs = d.rstd[(n0 + j) * d.G + l.g];
+            float aq[2] = {0.f, 0.f};
+            with_activation(d.act, [&](auto act) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (!live || l.row + k * step >= S) continue;
-                float h[V], dz[V];
-                back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
+                for (int k = 0; k < K; ++k) {
+                    if (!live || l.row + k * step >= S) continue;
+                    float h[V], dz[V];
+                    back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s1[i] += dz[i];
-                    s2[i] = fmaf(dz[i], h[i], s2[i]);
-                    aq[0] = fmaf(dz[i], w[i], aq[0]);
-                    aq[1] = fmaf(dz[i] * w[i], h[i], aq[1]);
+                    for (int i = 0; i < V; ++i) {
+                        s1[i] += dz[i];
+                        s2[i] = fmaf(dz[i], h[i], s2[i]);
+                        aq[0] = fmaf(dz[i], w[i], aq[0]);
+                        aq[1] = fmaf(dz[i] * w[i], h[i], aq[1]);
+                    }
                 }
-            }
-        });
-        group_sum<TH>(aq, d, TH == 64 ? scratch : scratch + turn * 2 * TH);
-        const float a = aq[0] * inv, q = aq[1] * inv;
-        const long out = n0 * d.S * d.C;
-        const int at = (j * S + l.row) * d.C + l.ch;
-        forget(xv);
-        forget(gv);
-        forget(rv);
-        with_activation(d.act, [&](auto act) {
+            });
+            group_sum<TH>(aq, d, TH == 64 ? scratch : scratch + turn * 2 * TH);
+            const float a = aq[0] * inv, q = aq[1] * inv;
+            const long out = n0 * d.S * d.C;
+            const int at = (j * S + l.row) * d.C + l.ch;
+            forget(xv);
+            forget(gv);
+            forget(rv);
+            with_activation(d.act, [&](auto act) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (!live || l.row + k * step >= S) continue;
-                float h[V], dz[V];
-                back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
-                back_store<T, V>(d, out, (unsigned)(at + k * step * d.C), rs, a, q, w, h, dz);
-            }
-        });
-    }
-    if (!d.dw && !d.db) continue;
-    column_sum<TH>(s1, d, scratch);
-    column_sum<TH>(s2, d, TH == 64 ? scratch : scratch + TH * V);
-    if (TH > 64) __syncthreads();                           // before another tile's sums
-    if (l.live && l.row == 0 && l.sample == 0) {
-        mz::store<float, V>(d.ws + block * 2 * d.C + l.ch, s1);
-        mz::store<float, V>(d.ws + block * 2 * d.C + d.C + l.ch, s2);
-    }
+                for (int k = 0; k < K; ++k) {
+                    if (!live || l.row + k * step >= S) continue;
+                    float h[V], dz[V];
+                    back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
+                    back_store<T, V>(d, out, (unsigned)(at + k * step * d.C), rs, a, q, w, h, dz);
+                }
+            });
+        }
+        if (!d.dw && !d.db) continue;
+        column_sum<TH>(s1, d, scratch);
+        column_sum<TH>(s2, d, TH == 64 ? scratch : scratch + TH * V);
+        if (TH > 64) __syncthreads();                           // before another tile's sums
+        if (l.live && l.row == 0 && l.sample == 0) {
+            mz::store<float, V>(d.ws + block * 2 * d.C + l.ch, s1);
+            mz::store<float, V>(d.ws + block * 2 * d.C + d.C + l.ch, s2);
+        }
     }
 }
 
@@ -652,7 +652,13 @@ __global__ void __launch_bounds__(1024) norm_params_kernel(Norm d, long rows) {
     const int t = threadIdx.x, c = blockIdx.x * 16 + (t & 15);
     double s = 0.0;
     if (c < 2 * d.C)
-        for (long r = t >> 4; r < rows; r += 64) s += d.ws[r * 2 * d.C + c];
+        for (long r = t >> 4; r < rows; r += 4 * 64) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = r + k * 64 < rows ? d.ws[(r + k * 64) * 2 * d.C + c] : 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += v[k];
+        }
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
     part[t] = s;
@@ -685,6 +691,7 @@ template <typename F>
 void with_size(const Plan& p, F f) {                // threads, and vectors a thread, of the resident kernels
     if (p.threads == 64) {
         if (p.k <= 2) f(Int<64>{}, Int<2>{});
+        else if (p.k <= 4) f(Int<64>{}, Int<4>{});
         else f(Int<64>{}, Int<8>{});
     } else if (p.threads == 256) {
         f(Int<256>{}, Int<8>{});
