@@ -65,6 +65,8 @@ const char* mz_last_error(void);
 int mz_version(void);
 /* Number of visible HIP devices (0 when there is none); never initialises a device context. */
 int mz_device_count(void);
+/* 1 while `stream` is being captured into a graph, 0 if not (the default stream never is). */
+int mz_stream_is_capturing(void* stream);
 
 /* ---- tree pool ------------------------------------------------------------------------------------ */
 

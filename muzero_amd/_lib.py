@@ -90,6 +90,7 @@ PROTOTYPES = {
     'mz_last_error': (ctypes.c_char_p, []),
     'mz_version': (ctypes.c_int, []),
     'mz_device_count': (ctypes.c_int, []),
+    'mz_stream_is_capturing': (ctypes.c_int, [c_void_p]),
     'mz_pool_create': (ctypes.c_int, [ctypes.POINTER(PoolConfig), c_void_p, ctypes.POINTER(c_void_p)]),
     'mz_pool_destroy': (ctypes.c_int, [c_void_p]),
     'mz_pool_set_stream': (ctypes.c_int, [c_void_p, c_void_p]),
@@ -170,6 +171,23 @@ PROTOTYPES = {
 }
 
 _lib = None
+
+
+_native = None
+
+
+def native():
+    """The autograd side of the training operators (csrc/mz_autograd.cpp, next to libmzhip.so)."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _autograd
+        except ImportError as e:
+            raise MuZeroError(f'muzero_amd/_autograd.so cannot be loaded ({e}): build it with '
+                              f'`python -c "import __graft_entry__ as g; g.build()"`') from e
+        _native = _autograd
+    return _native
 
 
 def load():

@@ -28,4 +28,11 @@ int mz_device_count(void) {
     return n;
 }
 
+int mz_stream_is_capturing(void* stream) {
+    if (!stream) return 0;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    MZ_HIP(hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status));
+    return status != hipStreamCaptureStatusNone;
+}
+
 }  // extern "C"

@@ -2,114 +2,22 @@
 global gradient norm and clipping by it (csrc/mz_clip.hip).  The reference leaves them to Keras (training.py:13-51,157-204);
 the names follow its framework."""
 import ctypes
-import math
 import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from ._launch import DTYPES, launch, once, refuse_capture_of_live_leaves, remember_leaves, require_hip, require_tensor
+from ._launch import DTYPES, launch, require_hip, require_tensor
 from .exceptions import MuZeroError
-
-MAX_CLASSES = 4096
 
 
 # ---- categorical loss ----------------------------------------------------------------------------------------------------
-# mz_categorical_t up to its dloss_strides, and those
-_CONFIG, _DLOSS = struct.Struct('=qqqqiiiiqqqq'), struct.Struct('=qq')
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _rows(t):
-    """A tensor of the rows' shape -> (t or a dense copy of it, unroll stride, batch stride)."""
-    if t.dim() == 2:
-        return (t, *t.stride())
-    return t.contiguous(), 0, 1
-
-
-def _describe(logits, targets, game, position, weights):
-    """Checks the arguments of a loss -> the tensors as the kernel reads them (logits, targets, game, position, weights) and
-    the configuration without dloss_strides."""
-    require_tensor('logits', logits, DTYPES)
-    device, shape = logits.device, logits.shape
-    if len(shape) < 2 or not 1 <= shape[-1] <= MAX_CLASSES:
-        raise MuZeroError(f'logits must be [..., classes] with 1 to {MAX_CLASSES} classes, got {tuple(shape)}')
-    require_tensor('targets', targets, (torch.float32,), device)
-    if targets.requires_grad:
-        raise MuZeroError('the loss is not differentiable with respect to targets')
-    rows, classes = shape[:-1], shape[-1]
-    index_bytes = 4
-    if game is not None or position is not None:
-        if len(shape) != 3:
-            raise MuZeroError(f'with game and position, logits must be [unroll, batch, classes], got {tuple(shape)}')
-        if game is None or position is None:
-            raise MuZeroError('game and position: both or neither')
-        if targets.dim() != 3 or targets.shape[-1] != classes:
-            raise MuZeroError(f'targets must be [positions, games, {classes}], got {tuple(targets.shape)}')
-        for name, t in (('game', game), ('position', position)):
-            require_tensor(name, t, (torch.int32, torch.int64), device)
-            if t.shape != rows[1:]:
-                raise MuZeroError(f'{name} must have shape ({rows[1]},), got {tuple(t.shape)}')
-        if game.dtype != position.dtype:
-            raise MuZeroError(f'game is {game.dtype}, position {position.dtype}: both must be of one type')
-        index_bytes = 4 if game.dtype == torch.int32 else 8
-        game, position = game.contiguous(), position.contiguous()
-        positions, games = targets.shape[:2]
-    elif targets.shape != shape:
-        raise MuZeroError(f'targets have shape {tuple(targets.shape)}, logits {tuple(shape)}')
-    else:
-        positions, games = rows if len(rows) == 2 else (1, math.prod(rows))
-    wu = wb = 0
-    if weights is not None:
-        require_tensor('weights', weights, (torch.float32,), device)
-        if weights.requires_grad:
-            raise MuZeroError('the loss is not differentiable with respect to weights')
-        if weights.shape != rows:
-            try:
-                weights = weights.expand(rows)
-            except RuntimeError:
-                raise MuZeroError(f'weights of shape {tuple(weights.shape)} do not broadcast to {tuple(rows)}') from None
-        weights, wu, wb = _rows(weights)
-    require_hip(device)
-    if len(rows) == 2:
-        if logits.stride(-1) != 1 and classes > 1:
-            logits = logits.contiguous()
-        (unroll, batch), (zu, zb, _) = rows, logits.stride()
-    else:
-        logits = logits.contiguous()
-        unroll, batch, zu, zb = 1, math.prod(rows), 0, classes
-    config = _CONFIG.pack(unroll, batch, positions, games, classes, DTYPES[logits.dtype], index_bytes, 0, zu, zb, wu, wb)
-    return (logits, targets.contiguous(), game, position, weights), config
-
-
-def _run(tensors, config, with_loss, with_grad, dloss=None):
-    logits, targets, game, position, weights = tensors
-    shape, device = logits.shape, logits.device
-    gu = gb = 0
-    if dloss is not None:
-        dloss, gu, gb = _rows(dloss)
-    loss = torch.empty(shape[:-1], dtype=torch.float32, device=device) if with_loss else None
-    grad = torch.empty(shape, dtype=logits.dtype, device=device) if with_grad else None
-    launch(device, _lib.load().mz_categorical_loss, config + _DLOSS.pack(gu, gb), logits.data_ptr(), targets.data_ptr(), _ptr(game),
-           _ptr(position), _ptr(weights), _ptr(dloss), _ptr(loss), _ptr(grad))
-    return loss, grad
-
-
-class _CategoricalLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tensors, config):
-        ctx.save_for_backward(*tensors)
-        ctx.config = config
-        return _run(tensors, config, True, False)[0]
-
-    @staticmethod
-    @once
-    def backward(ctx, dloss):
-        return _run(ctx.saved_tensors, ctx.config, False, True, dloss)[1], None, None
+def _loss(fn, *tensors):
+    try:
+        return fn(*tensors)
+    except TypeError:
+        raise MuZeroError('logits, targets, game, position and weights are tensors (the last three may be None)') from None
 
 
 def categorical_loss(logits: torch.Tensor, targets: torch.Tensor, game: Optional[torch.Tensor] = None,
@@ -123,11 +31,7 @@ def categorical_loss(logits: torch.Tensor, targets: torch.Tensor, game: Optional
     does not look at them).  weights broadcast over the rows; rows of weight 0 are not read and give 0 whatever they hold.  A
     class with target 0 adds nothing, also where its logit is -inf (an illegal move); a row whose logits are all -inf gives 0.
     A row of zero targets (past the end of a game) gives 0.  Differentiable once with respect to logits alone."""
-    tensors, config = _describe(logits, targets, game, position, weights)
-    if not torch.is_grad_enabled() or not logits.requires_grad:
-        return _run(tensors, config, True, False)[0]
-    refuse_capture_of_live_leaves(logits.device, (logits,))
-    return remember_leaves(logits.device, _CategoricalLoss.apply(logits, tensors, config))
+    return _loss(_lib.native().categorical_loss, logits, targets, game, position, weights)
 
 
 def categorical_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, game: Optional[torch.Tensor] = None,
@@ -136,8 +40,7 @@ def categorical_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, game:
     """-> (categorical_loss(...), the gradient of its sum with respect to logits, of their shape and type), in one launch
     and outside autograd: for a step whose factors are all in `weights` (importance of the samples, scale of the unrolled
     steps), which passes the gradient on with logits.backward(grad)."""
-    tensors, config = _describe(logits, targets, game, position, weights)
-    return _run(tensors, config, True, True)
+    return _loss(_lib.native().categorical_loss_and_grad, logits, targets, game, position, weights)
 
 
 # ---- global norm and clipping --------------------------------------------------------------------------------------------
