@@ -1,4 +1,4 @@
-// torch's side of group norm and the categorical loss: argument checks, strides, outputs and autograd nodes around the C
+// torch's side of group norm, the categorical loss and clipping: argument checks, strides, outputs and autograd nodes around the C
 // entries of libmzhip.so.  Built as muzero_amd/_autograd.so.  In C++ because a node in Python costs more than these
 // operators do: its backward pass runs on the autograd thread, has to take the interpreter from the thread that waits for
 // it, and moves Python's objects between the cores of both (120 to 130 us a forward and backward pass of a small state,
@@ -6,8 +6,11 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <string>
+#include <vector>
 
 #include "../../include/mzhip.h"
 
@@ -372,6 +375,135 @@ std::pair<Tensor, Tensor> categorical_loss_and_grad(const Tensor& logits, const 
     return loss_run(c, true, true, Tensor());
 }
 
+// ---- global norm and clipping -----------------------------------------------------------------------------------------
+
+// every element of t's memory span once: contiguous in some order of its dimensions
+bool dense(const Tensor& t) {
+    if (t.is_contiguous()) return true;
+    std::vector<std::pair<int64_t, int64_t>> dims;
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) != 1) dims.emplace_back(t.stride(i), t.size(i));
+    std::sort(dims.begin(), dims.end());
+    int64_t span = 1;
+    for (const auto& [stride, size] : dims) {
+        if (stride != span) return false;
+        span *= size;
+    }
+    return true;
+}
+
+struct TensorList {
+    std::vector<Tensor> tensors, out;
+    std::vector<mz_tensor_t> described;
+    std::vector<void*> outputs;
+    c10::Device device = at::kCPU;
+
+    TensorList(std::vector<Tensor> t, std::optional<std::vector<Tensor>> o) : tensors(std::move(t)) {
+        const size_t n = tensors.size();
+        if (n < 1 || n > MZ_GLOBAL_NORM_MAX_TENSORS) refuse("1 to ", MZ_GLOBAL_NORM_MAX_TENSORS, " tensors, got ", n);
+        device = tensors[0].device();
+        described.reserve(n);
+        for (size_t i = 0; i < n; ++i) {
+            const Tensor& t = tensors[i];
+            if (dtype_of(t) < 0) refuse("tensor ", i, ": expected float32, float16 or bfloat16, got ", t.scalar_type());
+            if (t.device() != device) refuse("tensor ", i, " is on ", t.device(), ", expected ", device);
+            if (!dense(t)) refuse("tensor ", i, " is not dense: shape ", t.sizes(), ", strides ", t.strides());
+            described.push_back({t.data_ptr(), t.numel(), dtype_of(t), 0});
+        }
+        if (o) {
+            out = std::move(*o);
+            if (out.size() != n) refuse(n, " tensors, ", out.size(), " outputs");
+            for (size_t i = 0; i < n; ++i) {
+                const Tensor &t = tensors[i], &u = out[i];
+                if (u.scalar_type() != t.scalar_type() || u.device() != device || u.sizes() != t.sizes() ||
+                    !((u.is_contiguous() && t.is_contiguous()) || u.strides() == t.strides()))
+                    refuse("output ", i, " must be like its tensor: ", t.scalar_type(), " ", t.sizes(), ", strides ", t.strides(), ", on ", device);
+                outputs.push_back(u.data_ptr());
+            }
+        }
+        require_hip(device);
+    }
+    const std::vector<Tensor>& written() const { return outputs.empty() ? tensors : out; }
+    void* const* output_table() const { return outputs.empty() ? nullptr : outputs.data(); }
+    void check_clip(double max_norm) const {
+        if (!(max_norm >= 0)) refuse("max_norm must be >= 0, got ", max_norm);
+        for (const Tensor& t : written())
+            if (t.requires_grad()) refuse("a tensor that requires grad cannot be written by clipping");
+    }
+    void changed() const {
+        for (const Tensor& t : written())
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    // call(stream, workspace, its size, norm) -> status
+    template <typename F>
+    Tensor run(F call) const {
+        const auto options = at::TensorOptions().device(device);
+        const Tensor ws = at::empty({MZ_GLOBAL_NORM_WORKSPACE}, options.dtype(at::kByte)), norm = at::empty({}, options.dtype(at::kFloat));
+        const On on(device);
+        done(call(on.stream, ws.data_ptr(), MZ_GLOBAL_NORM_WORKSPACE, norm.data_ptr<float>()));
+        return norm;
+    }
+};
+
+Tensor global_norm(std::vector<Tensor> tensors) {
+    const TensorList l(std::move(tensors), std::nullopt);
+    return l.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
+        return mz_global_norm(stream, (int32_t)l.described.size(), l.described.data(), ws, bytes, norm);
+    });
+}
+
+Tensor clip_by_global_norm(std::vector<Tensor> tensors, double max_norm, std::optional<std::vector<Tensor>> out) {
+    const TensorList l(std::move(tensors), std::move(out));
+    l.check_clip(max_norm);
+    const Tensor norm = l.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
+        return mz_clip_by_global_norm(stream, (int32_t)l.described.size(), l.described.data(), l.output_table(), max_norm, ws, bytes, norm);
+    });
+    l.changed();
+    return norm;
+}
+
+class GradientSet {
+    TensorList list_;
+    mz_tensor_table_t table_;
+    Tensor memory_;                              // the table on the device
+    c10::Stream made_on_;
+    std::string overlap_;
+
+    c10::Stream current() const { return c10::impl::VirtualGuardImpl(list_.device.type()).getStream(list_.device); }
+    void* table() const {
+        const c10::Stream stream = current();
+        if (stream != made_on_ && !done(mz_stream_is_capturing(On(list_.device).stream))) memory_.record_stream(stream);
+        return memory_.data_ptr();
+    }
+
+  public:
+    GradientSet(std::vector<Tensor> tensors, std::optional<std::vector<Tensor>> out)
+        : list_(std::move(tensors), std::move(out)), made_on_(current()) {
+        if (done(mz_stream_is_capturing(On(list_.device).stream))) refuse("a GradientSet uploads its table: make it before the capture");
+        const int32_t n = (int32_t)list_.described.size();
+        Tensor host = at::empty({(int64_t)n * MZ_TENSOR_TABLE_ENTRY}, at::kByte);
+        done(mz_tensor_table_build(n, list_.described.data(), list_.output_table(), host.data_ptr(), &table_));
+        if (!table_.writable) overlap_ = mz_last_error();
+        memory_ = host.to(list_.device);
+    }
+    Tensor global_norm() const {
+        void* const table = this->table();
+        return list_.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
+            return mz_tensor_table_global_norm(stream, &table_, table, ws, bytes, norm);
+        });
+    }
+    Tensor clip_by_global_norm(double max_norm) const {
+        list_.check_clip(max_norm);
+        if (!overlap_.empty()) refuse("cannot clip: ", overlap_);
+        void* const table = this->table();
+        const Tensor norm = list_.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
+            return mz_tensor_table_clip(stream, &table_, table, max_norm, ws, bytes, norm);
+        });
+        list_.changed();
+        return norm;
+    }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
@@ -390,4 +522,10 @@ PYBIND11_MODULE(_autograd, m) {
     m.def("group_norm", &group_norm, py::call_guard<py::gil_scoped_release>());
     m.def("categorical_loss", &categorical_loss, py::call_guard<py::gil_scoped_release>());
     m.def("categorical_loss_and_grad", &categorical_loss_and_grad, py::call_guard<py::gil_scoped_release>());
+    m.def("global_norm", &global_norm, py::call_guard<py::gil_scoped_release>());
+    m.def("clip_by_global_norm", &clip_by_global_norm, py::call_guard<py::gil_scoped_release>());
+    py::class_<GradientSet>(m, "GradientSet")
+        .def(py::init<std::vector<Tensor>, std::optional<std::vector<Tensor>>>(), py::call_guard<py::gil_scoped_release>())
+        .def("global_norm", &GradientSet::global_norm, py::call_guard<py::gil_scoped_release>())
+        .def("clip_by_global_norm", &GradientSet::clip_by_global_norm, py::call_guard<py::gil_scoped_release>());
 }

@@ -1,14 +1,11 @@
 """Operators of a training step on the targets of replay.py: the categorical loss with its gradient (csrc/mz_loss.hip), the
 global gradient norm and clipping by it (csrc/mz_clip.hip).  The reference leaves them to Keras (training.py:13-51,157-204);
 the names follow its framework."""
-import ctypes
-import struct
-from typing import List, Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from ._launch import DTYPES, launch, require_hip, require_tensor
 from .exceptions import MuZeroError
 
 
@@ -44,65 +41,11 @@ def categorical_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, game:
 
 
 # ---- global norm and clipping --------------------------------------------------------------------------------------------
-def _dense(t):
-    """Every element of t's memory span once: contiguous in some order of its dimensions."""
-    if t.is_contiguous():
-        return True
-    span = 1
-    for st, size in sorted((st, size) for st, size in zip(t.stride(), t.shape) if size != 1):
-        if st != span:
-            return False
-        span *= size
-    return True
-
-
-def _like(t, o):
-    return isinstance(o, torch.Tensor) and o.dtype == t.dtype and o.device == t.device and o.shape == t.shape and \
-        (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride())
-
-
-def _describe_tensors(tensors, out):
-    """Checks -> (device, mz_tensor_t array, output pointers or None)."""
-    n = len(tensors)
-    if not 1 <= n <= _lib.MZ_GLOBAL_NORM_MAX_TENSORS:
-        raise MuZeroError(f'1 to {_lib.MZ_GLOBAL_NORM_MAX_TENSORS} tensors, got {n}')
-    device = require_tensor('tensor 0', tensors[0], DTYPES).device
-    table = bytearray()
-    for i, t in enumerate(tensors):
-        if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES or t.device != device:
-            require_tensor(f'tensor {i}', t, DTYPES, device)
-        if not _dense(t):
-            raise MuZeroError(f'tensor {i} is not dense: shape {tuple(t.shape)}, strides {t.stride()}')
-        table += _TENSOR.pack(t.data_ptr(), t.numel(), DTYPES[t.dtype])
-    outputs = None
-    if out is not None:
-        if len(out) != n:
-            raise MuZeroError(f'{n} tensors, {len(out)} outputs')
-        for i, (t, o) in enumerate(zip(tensors, out)):
-            if not _like(t, o):
-                raise MuZeroError(f'output {i} must be like its tensor: {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}')
-        outputs = struct.pack(f'={n}Q', *[o.data_ptr() for o in out])
-    require_hip(device)
-    return device, bytes(table), outputs
-
-
-_TENSOR = struct.Struct('=Qqi4x')          # mz_tensor_t
-
-
-def _call(device, fn, *args):
-    """fn(stream, *args, workspace, its size, norm) -> norm"""
-    workspace = torch.empty(_lib.MZ_GLOBAL_NORM_WORKSPACE, dtype=torch.uint8, device=device)
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    launch(device, fn, *args, workspace.data_ptr(), _lib.MZ_GLOBAL_NORM_WORKSPACE, norm.data_ptr())
-    return norm
-
-
-def _check_clip(max_norm, written):
-    if not max_norm >= 0:
-        raise MuZeroError(f'max_norm must be >= 0, got {max_norm}')
-    for t in written:
-        if t.requires_grad:
-            raise MuZeroError('a tensor that requires grad cannot be written by clipping')
+def _list(fn, *args):
+    try:
+        return fn(*args)
+    except TypeError:
+        raise MuZeroError('tensors and out are lists of tensors (out may be None), max_norm is a number') from None
 
 
 class GradientSet:
@@ -116,59 +59,26 @@ class GradientSet:
     captures.  Results are ordered on the current stream; a set may be used on several streams at once."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None) -> None:
-        self.tensors: List[torch.Tensor] = list(tensors)
-        self.out = None if out is None else list(out)
-        self.device, described, outputs = _describe_tensors(self.tensors, self.out)
-        if torch.cuda.is_current_stream_capturing():
-            raise MuZeroError('a GradientSet uploads its table: make it before the capture')
-        self._lib = _lib.load()
-        n = len(self.tensors)
-        host = bytearray(n * _lib.MZ_TENSOR_TABLE_ENTRY)
-        self._table = _lib.TensorTable()
-        _lib.check(self._lib.mz_tensor_table_build(n, described, outputs, (ctypes.c_char * len(host)).from_buffer(host),
-                                                   ctypes.byref(self._table)))
-        self._overlap = None if self._table.writable else self._lib.mz_last_error().decode('utf-8', 'replace')
-        self._memory = torch.frombuffer(host, dtype=torch.uint8).to(self.device)
-        self._stream = torch.cuda.current_stream(self.device)
-
-    def _run(self, fn, *args):
-        stream = torch.cuda.current_stream(self.device)
-        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
-            self._memory.record_stream(stream)
-        return _call(self.device, fn, ctypes.byref(self._table), self._memory.data_ptr(), *args)
+        self._set = _list(_lib.native().GradientSet, list(tensors), None if out is None else list(out))
 
     def global_norm(self) -> torch.Tensor:
         """sqrt of the sum of the squares of all elements of all tensors: a float32 scalar on the device."""
-        return self._run(self._lib.mz_tensor_table_global_norm)
+        return self._set.global_norm()
 
     def clip_by_global_norm(self, max_norm: float) -> torch.Tensor:
         """Writes every tensor times max_norm / global norm to its output where the norm is above max_norm, else unchanged,
         and returns the norm before clipping.  Where that is NaN every output is NaN; where it is infinite, finite elements
         become 0 and infinite ones NaN."""
-        written = self.tensors if self.out is None else self.out
-        _check_clip(max_norm, written)
-        if self._overlap:
-            raise MuZeroError(f'cannot clip: {self._overlap}')
-        norm = self._run(self._lib.mz_tensor_table_clip, max_norm)
-        torch.autograd.graph.increment_version(written)
-        return norm
+        return _list(self._set.clip_by_global_norm, max_norm)
 
 
 def global_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     """GradientSet(tensors).global_norm() for tensors that are others in every step: their table travels with the launch, 112
     tensors each, and nothing is uploaded."""
-    tensors = list(tensors)
-    device, described, _ = _describe_tensors(tensors, None)
-    return _call(device, _lib.load().mz_global_norm, len(tensors), described)
+    return _list(_lib.native().global_norm, list(tensors))
 
 
 def clip_by_global_norm(tensors: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """GradientSet(tensors, out).clip_by_global_norm(max_norm) in the same way: in place, or into `out`; returns the norm
     before clipping.  Tensors that are written may not share memory with others of the list."""
-    tensors, out = list(tensors), None if out is None else list(out)
-    device, described, outputs = _describe_tensors(tensors, out)
-    written = tensors if out is None else out
-    _check_clip(max_norm, written)
-    norm = _call(device, _lib.load().mz_clip_by_global_norm, len(tensors), described, outputs, max_norm)
-    torch.autograd.graph.increment_version(written)
-    return norm
+    return _list(_lib.native().clip_by_global_norm, list(tensors), max_norm, None if out is None else list(out))
