@@ -8,8 +8,7 @@
 //
 // Bound by memory: logits and targets are read once, the gradient is written once.  A row belongs to W lanes (a power of
 // two), which hold all of it: up to K chunks of V adjacent classes each, read as one access a chunk, and two rounds of
-// shuffles: the maximum, then the three sums together.  A last chunk that would pass the row's end is moved back to end
-// with it; its first classes are its neighbour's too, which the sums leave out and the store writes a second time, alike.
+// shuffles: the maximum, then the three sums together.
 #include "mz_vec.h"
 #include <cmath>
 
@@ -21,10 +20,11 @@ using mz::Vec;
 
 constexpr int kThreads = 256;
 constexpr int kMaxClasses = 4096;
+constexpr float kLog2e = 1.4426950409f;
 
 struct Loss {
-    long U, B, P, G;
-    int C, wide, lanes, chunks;         // wide: 8-byte indexes; lanes of a row, chunks of a row
+    long U, B, P, G, u0;                // u0: first step of a launch
+    int C, wide, lanes, last;           // wide: 8-byte indexes; lanes of a row, a lane's last chunk
     long zs[2], ws[2], gs[2];
     const void* z;
     const float *t, *w, *g;
@@ -37,91 +37,123 @@ __device__ inline long index_at(const void* p, int wide, long i) {
     return wide ? (long)static_cast<const int64_t*>(p)[i] : (long)static_cast<const int32_t*>(p)[i];
 }
 
-template <typename T, int V, int K>
+// K chunks a lane: exactly K up to four, then up to K.
+template <typename T, int V, int K, bool LOSS, bool GRAD>
 __global__ void __launch_bounds__(kThreads) categorical_kernel(Loss d) {
-    const int lane = threadIdx.x & (d.lanes - 1);
-    const long per_block = kThreads / d.lanes;
-    for (long u = blockIdx.y; u < d.U; u += gridDim.y)
-        for (long b = blockIdx.x * per_block + threadIdx.x / d.lanes; b < d.B; b += gridDim.x * per_block) {
-            const T* z = static_cast<const T*>(d.z) + u * d.zs[0] + b * d.zs[1];
-            const float w = d.w ? d.w[u * d.ws[0] + b * d.ws[1]] : 1.f;
-            const long position = d.position ? index_at(d.position, d.wide, b) : 0, game = d.game ? index_at(d.game, d.wide, b) : b;
-            const bool inside = position >= 0 && position < d.P - u && game >= 0 && game < d.G;
-            const float* t = d.t + (inside ? ((position + u) * d.G + game) * d.C : 0);
-            Vec<T, V> zv[K];
-            Vec<float, V> tv[K];
-            float e[K][V], m = -INFINITY, sums[3] = {0.f, 0.f, 0.f};
-            if (w != 0.f && inside) {
+    const int lane = threadIdx.x & (d.lanes - 1), last = K <= 4 ? K - 1 : d.last;
+    const long u = d.u0 + blockIdx.y, b = blockIdx.x * (long)(kThreads / d.lanes) + threadIdx.x / d.lanes;
+    if (b >= d.B) return;                                    // all lanes of a row
+    // The lane's chunk k.  One that would pass the row's end is moved back to end with it: of the last chunk, the first `twice`
+    // classes belong to another lane (all V or more: the lane has no such chunk) and neither count nor are stored.
+    const auto start = [&](int k) { return (lane + k * d.lanes) * V < d.C - V ? (lane + k * d.lanes) * V : d.C - V; };
+    const int twice = (lane + last * d.lanes) * V - start(last);
+    const T* z = static_cast<const T*>(d.z) + u * d.zs[0] + b * d.zs[1];
+    Vec<T, V> zv[K];
+    Vec<float, V> tv[K];
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks) {
-                        const int c = (lane + k * d.lanes) * V < d.C - V ? (lane + k * d.lanes) * V : d.C - V;
-                        zv[k] = mz::load<T, V>(z + c);
-                        tv[k] = mz::load<float, V>(t + c);
-                    }
+    for (int k = 0; k < K; ++k)
+        if (k <= last) zv[k] = mz::load<T, V>(z + start(k));
+    const float w = d.w ? d.w[u * d.ws[0] + b * d.ws[1]] : 1.f;
+    const long position = d.position ? index_at(d.position, d.wide, b) : 0, game = d.game ? index_at(d.game, d.wide, b) : b;
+    const bool inside = position >= 0 && position < d.P - u && game >= 0 && game < d.G;
+    if (inside) {
+        const float* t = d.t + ((position + u) * d.G + game) * d.C;
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks)
+        for (int k = 0; k < K; ++k)
+            if (k <= last) tv[k] = mz::load<float, V>(t + start(k));
+    }
+    float e[K][V], m = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            e[k][i] = zv[k][i];
-                            m = fmaxf(m, e[k][i] != e[k][i] ? INFINITY : e[k][i]);      // a NaN ends in every sum
-                        }
-            }
-            for (int k = d.lanes >> 1; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-            const bool empty = w == 0.f || (inside && m == -INFINITY), live = inside && !empty;
-            if (live)
+    for (int k = 0; k < K; ++k)
+        if (k <= last) {
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks) {
-                        const int twice = (lane + k * d.lanes) * V - (d.C - V);         // classes that the neighbour counts
+            for (int i = 0; i < V; ++i) e[k][i] = zv[k][i];
+            if (k == last)
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const float below = m - e[k][i], q = tv[k][i];
-                            e[k][i] = __expf(-below);
-                            if (i >= twice) {
-                                sums[0] += e[k][i];
-                                sums[1] += q;
-                                if (q != 0.f) sums[2] = fmaf(q, below, sums[2]);
-                            }
-                        }
-                    }
-            for (int k = d.lanes >> 1; k; k >>= 1)
+                for (int i = 0; i < V; ++i) {
+                    e[k][i] = i < twice ? -INFINITY : e[k][i];
+                    tv[k].w[i] = i < twice ? 0 : tv[k].w[i];
+                }
 #pragma unroll
-                for (int i = 0; i < 3; ++i) sums[i] += __shfl_xor(sums[i], k);
-            const long row = u * d.B + b;
-            if (d.loss && lane == 0) d.loss[row] = empty ? 0.f : inside ? w * fmaf(sums[1], logf(sums[0]), sums[2]) : NAN;
-            if (d.grad) {
-                const float f = d.g ? w * d.g[u * d.gs[0] + b * d.gs[1]] : w, p = sums[1] / sums[0];
-                T* out = static_cast<T*>(d.grad) + row * d.C;
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (k * d.lanes < d.chunks && lane + k * d.lanes < d.chunks) {
-                        const int c = (lane + k * d.lanes) * V < d.C - V ? (lane + k * d.lanes) * V : d.C - V;
-                        float r[V];
-#pragma unroll
-                        for (int i = 0; i < V; ++i) r[i] = empty ? 0.f : inside ? f * fmaf(p, e[k][i], -tv[k][i]) : NAN;
-                        mz::store<T, V>(out + c, r);
-                    }
-            }
+            for (int i = 0; i < V; ++i) m = fmaxf(m, e[k][i]);
         }
+    for (int k = d.lanes >> 1; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    bool empty = w == 0.f;
+    if (m == -INFINITY) {                                    // nothing, or only NaN, above the lowest: a NaN is no empty row
+        float nan = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k <= last)
+#pragma unroll
+                for (int i = 0; i < V; ++i) nan += e[k][i] != e[k][i] ? 1.f : 0.f;
+        for (int k = d.lanes >> 1; k; k >>= 1) nan += __shfl_xor(nan, k);
+        empty |= inside && nan == 0.f;
+    }
+    const bool live = inside && !empty;
+    float s = 0.f, total = 0.f, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (k <= last)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float below = m - e[k][i];             // before the factor, which the type's lowest value would overflow
+                // a class without target adds nothing, also where its logit is -inf
+                if (LOSS) l = fmaf(tv[k][i], tv[k][i] != 0.f ? below : 0.f, l);
+                e[k][i] = __builtin_amdgcn_exp2f(below * -kLog2e);
+                s += e[k][i];
+                total += tv[k][i];
+            }
+    for (int k = d.lanes >> 1; k; k >>= 1) {
+        s += __shfl_xor(s, k);
+        total += __shfl_xor(total, k);
+        if (LOSS) l += __shfl_xor(l, k);
+    }
+    const long row = u * d.B + b;
+    if (LOSS && lane == 0) d.loss[row] = empty ? 0.f : inside ? w * fmaf(total, logf(s), l) : NAN;
+    if (GRAD) {
+        const float f = d.g ? w * d.g[u * d.gs[0] + b * d.gs[1]] : w, p = f * (total / s), dead = empty ? 0.f : NAN;
+        T* out = static_cast<T*>(d.grad) + row * d.C;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k <= last) {
+                float r[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) r[i] = live ? fmaf(p, e[k][i], -f * tv[k][i]) : dead;
+                if (k < last || twice <= 0) mz::store<T, V>(out + start(k), r);
+                else
+#pragma unroll
+                    for (int i = 1; i < V; ++i)
+                        if (i >= twice) out[start(k) + i] = (T)r[i];
+            }
+    }
+}
+
+template <typename T, int V, int K>
+void launch(const Loss& d, dim3 grid, hipStream_t st) {
+    if (d.loss && d.grad) categorical_kernel<T, V, K, true, true><<<grid, kThreads, 0, st>>>(d);
+    else if (d.loss) categorical_kernel<T, V, K, true, false><<<grid, kThreads, 0, st>>>(d);
+    else categorical_kernel<T, V, K, false, true><<<grid, kThreads, 0, st>>>(d);
 }
 
 template <typename T>
 void launch(Loss d, hipStream_t st) {
     // four classes a chunk, two chunks a lane; more chunks only where a wavefront's lanes are used up
-    const int v = d.C >= 4 ? 4 : 1;
-    d.chunks = (d.C + v - 1) / v;
+    const int v = d.C >= 4 ? 4 : 1, chunks = (d.C + v - 1) / v;
     d.lanes = 1;
-    while (d.lanes < 64 && d.lanes * 2 < d.chunks) d.lanes <<= 1;
-    const int k = (d.chunks + d.lanes - 1) / d.lanes;
-    const long blocks = (d.B + kThreads / d.lanes - 1) / (kThreads / d.lanes);
-    const dim3 grid((unsigned)(blocks < 1L << 20 ? blocks : 1L << 20), (unsigned)(d.U < 65535 ? d.U : 65535));
-    if (v == 1) categorical_kernel<T, 1, 2><<<grid, kThreads, 0, st>>>(d);
-    else if (k <= 2) categorical_kernel<T, 4, 2><<<grid, kThreads, 0, st>>>(d);
-    else if (k <= 4) categorical_kernel<T, 4, 4><<<grid, kThreads, 0, st>>>(d);
-    else if (k <= 8) categorical_kernel<T, 4, 8><<<grid, kThreads, 0, st>>>(d);
-    else categorical_kernel<T, 4, 16><<<grid, kThreads, 0, st>>>(d);
+    while (d.lanes < 64 && d.lanes * 2 < chunks) d.lanes <<= 1;
+    const int k = (chunks + d.lanes - 1) / d.lanes;
+    d.last = k - 1;
+    const long rows = kThreads / d.lanes;
+    for (; d.u0 < d.U; d.u0 += 65535) {                        // steps that a grid may hold
+        const dim3 grid((unsigned)((d.B + rows - 1) / rows), (unsigned)(d.U - d.u0 < 65535 ? d.U - d.u0 : 65535));
+        if (v == 1) k == 1 ? launch<T, 1, 1>(d, grid, st) : launch<T, 1, 2>(d, grid, st);
+        else if (k == 1) launch<T, 4, 1>(d, grid, st);
+        else if (k == 2) launch<T, 4, 2>(d, grid, st);
+        else if (k == 3) launch<T, 4, 3>(d, grid, st);
+        else if (k == 4) launch<T, 4, 4>(d, grid, st);
+        else if (k <= 8) launch<T, 4, 8>(d, grid, st);
+        else launch<T, 4, 16>(d, grid, st);
+    }
 }
 
 }  // namespace
@@ -138,6 +170,7 @@ extern "C" int mz_categorical_loss(void* stream, const mz_categorical_t* c, cons
     MZ_REQUIRE(c->target_games == 0 || c->target_positions <= (int64_t(1) << 48) / c->classes / c->target_games,
                "the targets have more than 2^48 elements");
     if (c->unroll == 0 || c->batch == 0) return MZ_OK;
+    MZ_REQUIRE(c->batch <= int64_t(1) << 31 && c->unroll <= int64_t(1) << 31, "more than 2^31 rows of a step, or steps");
     MZ_REQUIRE(logits && (targets || c->target_positions * c->target_games == 0), "logits/targets is NULL");
     if (!out_loss && !out_dlogits) return MZ_OK;
     Loss d = {};
@@ -162,7 +195,7 @@ extern "C" int mz_categorical_loss(void* stream, const mz_categorical_t* c, cons
     d.grad = out_dlogits;
     // rows that lie evenly behind one another, each with its own target row, are one long step
     const auto even = [&](const long* stride) { return stride[0] == d.B * stride[1]; };
-    if (!game && !position && d.P == d.U && d.G == d.B && even(d.zs) && (!d.w || even(d.ws)) && (!d.g || even(d.gs))) {
+    if (!game && !position && d.P == d.U && d.G == d.B && d.U * d.B <= 1L << 31 && even(d.zs) && (!d.w || even(d.ws)) && (!d.g || even(d.gs))) {
         d.B *= d.U;
         d.G = d.B;
         d.U = d.P = 1;
