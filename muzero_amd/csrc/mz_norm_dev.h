@@ -398,23 +398,31 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
 
 // ---- split ------------------------------------------------------------------------------------------------------------
 
+// A grid of (chunks, tiles, samples); f(sample, its chunk's first and last position, lane) for each of a workgroup's parts.
 struct Part {
     long n, s0, s1;
     int split, tile;
 };
-__device__ inline Part part_of(const Norm& d, long id) {
-    Part p;
-    p.tile = (int)(id % d.tiles);
-    id /= d.tiles;
-    p.split = (int)(id % d.splits);
-    p.n = id / d.splits;
-    p.s0 = p.split * d.chunk;
-    p.s1 = p.s0 + d.chunk < d.S ? p.s0 + d.chunk : d.S;
-    return p;
+template <typename F>
+__device__ inline void for_each_part(const Norm& d, F f) {
+    for (long n = blockIdx.z; n < d.N; n += gridDim.z)
+        for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y) {
+            const long s0 = blockIdx.x * d.chunk;
+            f(Part{n, s0, s0 + d.chunk < d.S ? s0 + d.chunk : d.S, (int)blockIdx.x, tile});
+        }
 }
 // where (split, piece) of a group stands among its splits * pieces partial results
 __device__ inline long part_at(const Norm& d, const Part& p, const Lane& l) {
     return ((p.n * d.G + l.g) * d.splits + p.split) * d.pieces + (d.pieces > 1 ? p.tile % d.pieces : 0);
+}
+
+constexpr int kBatch = 4;                       // vectors of a thread under way at once
+
+// vectors of positions s, s + step, ...; past the end the first again, which counts nothing
+template <typename T, int V>
+__device__ inline void load_batch(Vec<T, V> (&v)[kBatch], const T* p, long stride, long s, int step, long end) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) v[k] = mz::load<T, V>(p + (s + k * step < end ? s + k * step : s) * stride);
 }
 
 // ws [N][G][splits][pieces][2]: mean and sum of squared deviations of each part
@@ -422,34 +430,32 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kSplitThreads) norm_stats_kernel(Norm d) {
     __shared__ float scratch[2][kSplitThreads];
     const int step = 1 << d.lrows;
-    const long total = d.N * d.tiles * d.splits;
-    for (long id = blockIdx.x; id < total; id += gridDim.x) {
-        const Part p = part_of(d, id);
+    for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
         float count = 0.f, mean = 0.f, m2 = 0.f;
         if (l.live) {
             const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
-            constexpr int U = 4;
-            for (long s = p.s0 + l.row; s < p.s1; s += U * step) {     // U vectors on their own, then merged
-                Vec<T, V> v[U];
-#pragma unroll
-                for (int k = 0; k < U; ++k) v[k] = mz::load<T, V>(x + (s + k * step < p.s1 ? s + k * step : s) * d.xs[1]);
+            for (long s = p.s0 + l.row; s < p.s1; s += kBatch * step) {     // a batch on its own, then merged
+                Vec<T, V> v[kBatch];
+                load_batch(v, x, d.xs[1], s, step, p.s1);
                 float sum = 0.f, more = 0.f, dev = 0.f;
 #pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const bool in = s + k * step < p.s1;
-                    more += in ? (float)V : 0.f;
+                for (int k = 0; k < kBatch; ++k) {
+                    float q = 0.f;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) sum += in ? v[k][i] : 0.f;
+                    for (int i = 0; i < V; ++i) q += v[k][i];
+                    const bool in = s + k * step < p.s1;
+                    sum += in ? q : 0.f;
+                    more += in ? (float)V : 0.f;
                 }
                 const float m = sum / more;
 #pragma unroll
-                for (int k = 0; k < U; ++k)
+                for (int k = 0; k < kBatch; ++k) {
+                    float q = 0.f;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float e = s + k * step < p.s1 ? v[k][i] - m : 0.f;
-                        dev = fmaf(e, e, dev);
-                    }
+                    for (int i = 0; i < V; ++i) q = fmaf(v[k][i] - m, v[k][i] - m, q);
+                    dev += s + k * step < p.s1 ? q : 0.f;
+                }
                 const float e = m - mean, f = more / (count + more);
                 mean = fmaf(e, f, mean);
                 m2 += dev + e * e * count * f;
@@ -467,7 +473,7 @@ __global__ void __launch_bounds__(kSplitThreads) norm_stats_kernel(Norm d) {
             ws[0] = mu;
             ws[1] = v[0];
         }
-    }
+    });
 }
 
 template <typename T, int V>
@@ -475,55 +481,48 @@ __global__ void __launch_bounds__(kSplitThreads) norm_apply_kernel(Norm d) {
     __shared__ float scratch[2][kSplitThreads];
     const int step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
-    const long total = d.N * d.tiles * d.splits;
-    for (long id = blockIdx.x; id < total; id += gridDim.x) {
-        const Part p = part_of(d, id);
+    for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
         const long ng = p.n * d.G + l.g;
+        const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
+        const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
         // the group's parts, over its lanes (a part's share of the values: its positions times its vectors)
         const float* ws = d.ws + 2 * ng * d.splits * d.pieces;
         const int parts = d.splits * d.pieces, lanes = 1 << (d.ldv + d.lrows), mine = (l.row << d.ldv) + l.vec;
         const auto count = [&](int e) {
-            const int split = e / d.pieces, piece = e - split * d.pieces, left = d.D / V - (piece << d.ldv);
+            const int split = d.pieces > 1 ? e / d.pieces : e, piece = e - split * d.pieces, left = d.D / V - (piece << d.ldv);
             const long positions = split * d.chunk + d.chunk < d.S ? d.chunk : d.S - split * d.chunk;
             return (float)positions * (float)((left < 1 << d.ldv ? left : 1 << d.ldv) * V);
         };
-        float v[1] = {0.f};
+        float a[1] = {0.f};
         if (l.group < d.gs)
-            for (int e = mine; e < parts; e += lanes) v[0] = fmaf(count(e), ws[2 * e], v[0]);
-        group_sum<kSplitThreads>(v, d, scratch[0]);
-        const float mu = v[0] * inv;
-        v[0] = 0.f;
+            for (int e = mine; e < parts; e += lanes) a[0] = fmaf(count(e), ws[2 * e], a[0]);
+        group_sum<kSplitThreads>(a, d, scratch[0]);
+        const float mu = a[0] * inv;
+        a[0] = 0.f;
         if (l.group < d.gs)
-            for (int e = mine; e < parts; e += lanes) v[0] += fmaf(count(e) * (ws[2 * e] - mu), ws[2 * e] - mu, ws[2 * e + 1]);
-        group_sum<kSplitThreads>(v, d, scratch[1]);
-        const float rs = 1.f / sqrtf(v[0] * inv + d.eps);
-        if (!l.live) continue;
+            for (int e = mine; e < parts; e += lanes) a[0] += fmaf(count(e) * (ws[2 * e] - mu), ws[2 * e] - mu, ws[2 * e + 1]);
+        group_sum<kSplitThreads>(a, d, scratch[1]);
+        const float rs = 1.f / sqrtf(a[0] * inv + d.eps);
+        if (!l.live) return;
         if (d.mean && p.split == 0 && l.vec == 0 && l.row == 0 && (d.pieces == 1 || p.tile % d.pieces == 0)) {
             d.mean[ng] = mu;
             d.rstd[ng] = rs;
         }
         float w[V], b[V];
         load_params<T, V>(d, l.ch, w, b);
-        const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
-        const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
         T* y = static_cast<T*>(d.y) + p.n * d.S * d.C + l.ch;
         with_activation(d.act, [&](auto act) {
-            constexpr int U = 4;
-            for (long s = p.s0 + l.row; s < p.s1; s += U * step) {
-                Vec<T, V> v[U], r[U];
+            for (long s = p.s0 + l.row; s < p.s1; s += kBatch * step) {
+                Vec<T, V> v[kBatch], r[kBatch];
+                load_batch(v, x, d.xs[1], s, step, p.s1);
+                if (res) load_batch(r, res, d.rs[1], s, step, p.s1);
 #pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const long at = s + k * step < p.s1 ? s + k * step : s;
-                    v[k] = mz::load<T, V>(x + at * d.xs[1]);
-                    if (res) r[k] = mz::load<T, V>(res + at * d.rs[1]);
-                }
-#pragma unroll
-                for (int k = 0; k < U; ++k)
+                for (int k = 0; k < kBatch; ++k)
                     if (s + k * step < p.s1) apply<T, V>(v[k], res ? &r[k] : nullptr, mu, rs, w, b, act, y + (s + k * step) * d.C);
             }
         });
-    }
+    });
 }
 
 // ws: sums of dz and dz h of a chunk's positions, [N * splits][2][C], then sums of dz w and dz w h of each part,
@@ -532,9 +531,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
     __shared__ float scratch[2][kSplitThreads * (V > 2 ? V : 2)];
     const int step = 1 << d.lrows;
-    const long total = d.N * d.tiles * d.splits;
-    for (long id = blockIdx.x; id < total; id += gridDim.x) {
-        const Part p = part_of(d, id);
+    for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
         const long ng = p.n * d.G + l.g;
         float s1[V] = {}, s2[V] = {}, w[V], b[V];
@@ -545,18 +542,13 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
             const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
             const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
             with_activation(d.act, [&](auto act) {
-                constexpr int U = 4;
-                for (long s = p.s0 + l.row; s < p.s1; s += U * step) {
-                    Vec<T, V> v[U], g[U], r[U];
+                for (long s = p.s0 + l.row; s < p.s1; s += kBatch * step) {
+                    Vec<T, V> v[kBatch], g[kBatch], r[kBatch];
+                    load_batch(v, x, d.xs[1], s, step, p.s1);
+                    load_batch(g, dy, d.ds[1], s, step, p.s1);
+                    if (res) load_batch(r, res, d.rs[1], s, step, p.s1);
 #pragma unroll
-                    for (int k = 0; k < U; ++k) {
-                        const long at = s + k * step < p.s1 ? s + k * step : s;
-                        v[k] = mz::load<T, V>(x + at * d.xs[1]);
-                        g[k] = mz::load<T, V>(dy + at * d.ds[1]);
-                        if (res) r[k] = mz::load<T, V>(res + at * d.rs[1]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < U; ++k) {
+                    for (int k = 0; k < kBatch; ++k) {
                         if (s + k * step >= p.s1) continue;
                         float h[V], dz[V];
                         back_values<T, V>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
@@ -589,7 +581,7 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
                 at[1] = aq[1];
             }
         }
-    }
+    });
 }
 
 template <typename T, int V>
@@ -597,12 +589,13 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
     __shared__ float scratch[2][2 * kSplitThreads];
     const int step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
-    const long total = d.N * d.tiles * d.splits;
     int turn = 0;
-    for (long id = blockIdx.x; id < total; id += gridDim.x, turn ^= 1) {
-        const Part p = part_of(d, id);
+    for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
         const long ng = p.n * d.G + l.g;
+        const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
+        const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
+        const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
         const float* ws = d.ws + d.N * d.splits * 2 * d.C + 2 * ng * d.splits * d.pieces;
         float aq[2] = {0.f, 0.f};
         if (l.group < d.gs)
@@ -611,27 +604,20 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
                 aq[1] += ws[2 * e + 1];
             }
         group_sum<kSplitThreads>(aq, d, scratch[turn]);
-        if (!l.live) continue;
+        turn ^= 1;
+        if (!l.live) return;
         const float mu = d.mean[ng], rs = d.rstd[ng], a = aq[0] * inv, q = aq[1] * inv;
         float w[V], b[V];
         load_params<T, V>(d, l.ch, w, b);
-        const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
-        const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
-        const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
         const long out = p.n * d.S * d.C + l.ch;
         with_activation(d.act, [&](auto act) {
-            constexpr int U = 4;
-            for (long s = p.s0 + l.row; s < p.s1; s += U * step) {
-                Vec<T, V> v[U], g[U], r[U];
+            for (long s = p.s0 + l.row; s < p.s1; s += kBatch * step) {
+                Vec<T, V> v[kBatch], g[kBatch], r[kBatch];
+                load_batch(v, x, d.xs[1], s, step, p.s1);
+                load_batch(g, dy, d.ds[1], s, step, p.s1);
+                if (res) load_batch(r, res, d.rs[1], s, step, p.s1);
 #pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const long at = s + k * step < p.s1 ? s + k * step : s;
-                    v[k] = mz::load<T, V>(x + at * d.xs[1]);
-                    g[k] = mz::load<T, V>(dy + at * d.ds[1]);
-                    if (res) r[k] = mz::load<T, V>(res + at * d.rs[1]);
-                }
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
+                for (int k = 0; k < kBatch; ++k) {
                     if (s + k * step >= p.s1) continue;
                     float h[V], dz[V];
                     back_values<T, V>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
@@ -639,7 +625,7 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
                 }
             }
         });
-    }
+    });
 }
 
 // ---- dweight, dbias ---------------------------------------------------------------------------------------------------
@@ -710,7 +696,7 @@ void forward(const Plan& p, int v, hipStream_t st) {
             const dim3 grid(grid_of((d.N + d.samples - 1) / d.samples), d.tiles < 65535 ? d.tiles : 65535);
             with_size(p, [&](auto th, auto k) { norm_forward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
         } else {
-            const unsigned grid = grid_of(d.N * d.tiles * d.splits);
+            const dim3 grid(d.splits, d.tiles < 65535 ? d.tiles : 65535, d.N < 65535 ? d.N : 65535);
             norm_stats_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
             norm_apply_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
         }
@@ -728,7 +714,7 @@ void backward(const Plan& p, int v, hipStream_t st) {
                 const dim3 grid((unsigned)d.blocks, d.tiles < 65535 ? d.tiles : 65535);
                 with_size(p, [&](auto th, auto k) { norm_backward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
             } else {
-                const unsigned grid = grid_of(d.N * d.tiles * d.splits);
+                const dim3 grid(d.splits, d.tiles < 65535 ? d.tiles : 65535, d.N < 65535 ? d.N : 65535);
                 norm_back_sums_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
                 if (d.dx || d.dres) norm_back_apply_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
             }
