@@ -583,7 +583,7 @@ int mz_clip_by_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, 
 typedef struct mz_tensor_table {
     int32_t entries, chunks;
     int64_t chunk;
-    int32_t writable, reserved;
+    int32_t writable, large;        /* large: more bytes than the last-level cache holds */
 } mz_tensor_table_t;
 int mz_tensor_table_build(int32_t n, const mz_tensor_t* tensors, void* const* outputs, void* host_table,
                           mz_tensor_table_t* out_table);

@@ -76,7 +76,7 @@ class Tensor(ctypes.Structure):
 
 class TensorTable(ctypes.Structure):
     """mz_tensor_table_t"""
-    _fields_ = [('entries', c_int32), ('chunks', c_int32), ('chunk', c_int64), ('writable', c_int32), ('reserved', c_int32)]
+    _fields_ = [('entries', c_int32), ('chunks', c_int32), ('chunk', c_int64), ('writable', c_int32), ('large', c_int32)]
 
 
 MZ_F32, MZ_F16, MZ_BF16 = 0, 1, 2

@@ -63,8 +63,8 @@ __device__ inline int tensor_of(const Entry* e, int n, int chunk) {
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// f(element index, values) over n elements at p, U vectors a thread under way at once
-template <typename T, typename F, typename G>
+// vector(index, values) and single(index) over n elements at p, U vectors a thread under way at once
+template <bool STREAM, typename T, typename F, typename G>
 __device__ inline void walk(const T* p, long n, F vector, G single) {
     constexpr int V = 16 / sizeof(T), U = 4;
     const long whole = n / V;
@@ -72,7 +72,7 @@ __device__ inline void walk(const T* p, long n, F vector, G single) {
         Vec<T, V> v[U];
 #pragma unroll
         for (int k = 0; k < U; ++k)
-            if (i + k * kThreads < whole) v[k] = mz::load<T, V>(p + (i + k * kThreads) * V);
+            if (i + k * kThreads < whole) v[k] = STREAM ? mz::load_streaming<T, V>(p + (i + k * kThreads) * V) : mz::load<T, V>(p + (i + k * kThreads) * V);
 #pragma unroll
         for (int k = 0; k < U; ++k)
             if (i + k * kThreads < whole) vector((i + k * kThreads) * V, v[k]);
@@ -80,10 +80,10 @@ __device__ inline void walk(const T* p, long n, F vector, G single) {
     for (long i = whole * V + threadIdx.x; i < n; i += kThreads) single(i);
 }
 
-template <typename T>
+template <bool STREAM, typename T>
 __device__ inline double squares(const T* p, long n) {
     double s = 0.0;
-    walk(p, n,
+    walk<STREAM>(p, n,
          [&](long, const Vec<T, 16 / sizeof(T)>& v) {
 #pragma unroll
              for (int k = 0; k < (int)(16 / sizeof(T)); ++k) s = fma((double)v[k], (double)v[k], s);
@@ -92,7 +92,10 @@ __device__ inline double squares(const T* p, long n) {
     return s;
 }
 
-template <typename Table>
+// STREAM: tensors that no cache holds until clipping reads them again.  At 1 GB that made this pass 206 -> 148 us, as it no
+// longer has to write back what the last clipping left there, and clipping 394 -> 423; at 63 MB, which a cache holds, it
+// made clipping 23 -> 31.
+template <typename Table, bool STREAM>
 __global__ void __launch_bounds__(kThreads) norm_partials_kernel(Table t, double* partials) {
     __shared__ double scratch[kThreads / 64];
     const Entry* e = t.entries();
@@ -100,9 +103,9 @@ __global__ void __launch_bounds__(kThreads) norm_partials_kernel(Table t, double
     for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
         const int i = tensor_of(e, t.n, chunk);
         const long at = (chunk - e[i].first) * t.chunk, n = e[i].elements - at < t.chunk ? e[i].elements - at : t.chunk;
-        if (e[i].dtype == MZ_F32) s += squares(static_cast<const float*>(e[i].in) + at, n);
-        else if (e[i].dtype == MZ_F16) s += squares(static_cast<const f16*>(e[i].in) + at, n);
-        else s += squares(static_cast<const bf16*>(e[i].in) + at, n);
+        if (e[i].dtype == MZ_F32) s += squares<STREAM>(static_cast<const float*>(e[i].in) + at, n);
+        else if (e[i].dtype == MZ_F16) s += squares<STREAM>(static_cast<const f16*>(e[i].in) + at, n);
+        else s += squares<STREAM>(static_cast<const bf16*>(e[i].in) + at, n);
     }
     s = mz::block_sum<kThreads>(s, scratch);
     if (threadIdx.x == 0) partials[blockIdx.x] = s;
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double* par
 
 template <typename T>
 __device__ inline void scale_chunk(const T* in, T* out, long n, float f) {
-    walk(in, n,
+    walk<false>(in, n,
          [&](long i, const Vec<T, 16 / sizeof(T)>& v) {
              float r[16 / sizeof(T)];
 #pragma unroll
@@ -132,7 +135,6 @@ __device__ inline void scale_chunk(const T* in, T* out, long n, float f) {
          [&](long i) { out[i] = (T)((float)in[i] * f); });
 }
 
-// Chunks from the last to the first: what the norm read last is what the caches still hold.
 template <typename Table>
 __global__ void __launch_bounds__(kThreads) clip_kernel(Table t, const double* partials, int n, double max_norm, float* out_norm) {
     __shared__ double scratch[kThreads / 64];
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(Table t, const double* p
     const double norm = norm_of(partials, n, scratch);
     if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) *out_norm = (float)norm;
     const float f = norm <= max_norm ? 1.f : (float)(max_norm / norm);        // a NaN norm gives NaN
-    for (int chunk = t.chunks - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
+    for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
         const int i = tensor_of(e, t.n, chunk);
         if (f == 1.f && e[i].in == e[i].out) continue;                        // nothing to change in place
         const long at = (chunk - e[i].first) * t.chunk, m = e[i].elements - at < t.chunk ? e[i].elements - at : t.chunk;
@@ -152,18 +154,24 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(Table t, const double* p
 
 // ---- host -------------------------------------------------------------------------------------------------------------
 
-int check(int32_t n, const mz_tensor_t* tensors, int64_t* total) {
+struct Total {
+    int64_t elements, bytes;
+};
+constexpr int64_t kCache = int64_t(1) << 28;               // bytes of the last-level cache
+
+int check(int32_t n, const mz_tensor_t* tensors, Total* total) {
     MZ_REQUIRE(n >= 1 && n <= MZ_GLOBAL_NORM_MAX_TENSORS, "between 1 and %d tensors, got %d", MZ_GLOBAL_NORM_MAX_TENSORS, n);
     MZ_REQUIRE(tensors, "tensors is NULL");
-    *total = 0;
+    *total = {0, 0};
     for (int32_t i = 0; i < n; ++i) {
         const int item = mz::dtype_size(tensors[i].dtype);
         MZ_REQUIRE(item, "tensor %d: dtype %d is not one of mz_dtype", i, tensors[i].dtype);
-        MZ_REQUIRE(tensors[i].elements >= 0 && tensors[i].elements <= kMost - *total, "tensor %d: %lld elements (2^43 in all at most)", i,
+        MZ_REQUIRE(tensors[i].elements >= 0 && tensors[i].elements <= kMost - total->elements, "tensor %d: %lld elements (2^43 in all at most)", i,
                    (long long)tensors[i].elements);
         MZ_REQUIRE(tensors[i].data || !tensors[i].elements, "tensor %d: data is NULL", i);
         MZ_REQUIRE((uintptr_t)tensors[i].data % item == 0, "tensor %d: data is not aligned to its type", i);
-        *total += tensors[i].elements;
+        total->elements += tensors[i].elements;
+        total->bytes += tensors[i].elements * item;
     }
     return MZ_OK;
 }
@@ -225,10 +233,10 @@ int chunks_of(int64_t elements, long chunk) { return (int)((elements + chunk - 1
 
 // Calls f(table, workgroups) for every launch's part of the tensors; empty tensors are left out.
 template <typename F>
-void for_each_table(int32_t n, const mz_tensor_t* tensors, void* const* outputs, int64_t total, F f) {
+void for_each_table(int32_t n, const mz_tensor_t* tensors, void* const* outputs, const Total& total, F f) {
     InArguments t;
     t.n = t.chunks = 0;
-    t.chunk = chunk_of(total);
+    t.chunk = chunk_of(total.elements);
     const int launches = (n + kBatch - 1) / kBatch;            // their workgroups share the room for partial sums
     const int most = kPartials / launches < kBlocks ? kPartials / launches : kBlocks;
     for (int32_t i = 0; i < n; ++i) {
@@ -249,10 +257,15 @@ int launched(const char* what) {
     return MZ_OK;
 }
 
-int partials_of(hipStream_t st, int32_t n, const mz_tensor_t* tensors, int64_t total, double* partials) {
+template <typename Table>
+void launch_partials(const Table& t, int grid, bool stream, hipStream_t st, double* partials) {
+    if (stream) norm_partials_kernel<Table, true><<<grid, kThreads, 0, st>>>(t, partials);
+    else norm_partials_kernel<Table, false><<<grid, kThreads, 0, st>>>(t, partials);
+}
+int partials_of(hipStream_t st, int32_t n, const mz_tensor_t* tensors, const Total& total, double* partials) {
     int used = 0;
     for_each_table(n, tensors, nullptr, total, [&](const InArguments& t, int grid) {
-        norm_partials_kernel<<<grid, kThreads, 0, st>>>(t, partials + used);
+        launch_partials(t, grid, total.bytes > kCache, st, partials + used);
         used += grid;
     });
     return used;
@@ -274,7 +287,7 @@ int blocks_of(const mz_tensor_table_t* t) { return t->chunks < kBlocks ? t->chun
 extern "C" {
 
 int mz_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* workspace, int64_t workspace_bytes, float* out_norm) {
-    int64_t total;
+    Total total;
     int bad = check(n, tensors, &total);
     if (!bad) bad = check_workspace(workspace, workspace_bytes, out_norm);
     if (bad) return bad;
@@ -287,7 +300,7 @@ int mz_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* wo
 
 int mz_clip_by_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, void* const* outputs, double max_norm,
                            void* workspace, int64_t workspace_bytes, float* out_norm) {
-    int64_t total;
+    Total total;
     int bad = check(n, tensors, &total);
     if (!bad) bad = check_workspace(workspace, workspace_bytes, out_norm);
     if (!bad) bad = check_written(n, tensors, outputs);
@@ -306,13 +319,14 @@ int mz_clip_by_global_norm(void* stream, int32_t n, const mz_tensor_t* tensors, 
 }
 
 int mz_tensor_table_build(int32_t n, const mz_tensor_t* tensors, void* const* outputs, void* host_table, mz_tensor_table_t* out_table) {
-    int64_t total;
+    Total total;
     const int bad = check(n, tensors, &total);
     if (bad) return bad;
     MZ_REQUIRE(host_table && out_table, "host_table/out_table is NULL");
     Entry* e = static_cast<Entry*>(host_table);
     mz_tensor_table_t t = {};
-    t.chunk = chunk_of(total);
+    t.chunk = chunk_of(total.elements);
+    t.large = total.bytes > kCache;
     // a table that clipping may not write still serves the norm
     t.writable = check_written(n, tensors, outputs) == MZ_OK;
     for (int32_t i = 0; i < n; ++i) {
@@ -332,7 +346,7 @@ int mz_tensor_table_global_norm(void* stream, const mz_tensor_table_t* table, co
     const hipStream_t st = static_cast<hipStream_t>(stream);
     double* partials = static_cast<double*>(workspace);
     const int blocks = blocks_of(table);
-    if (blocks) norm_partials_kernel<<<blocks, kThreads, 0, st>>>(in_memory(table, device_table), partials);
+    if (blocks) launch_partials(in_memory(table, device_table), blocks, table->large, st, partials);
     norm_finish_kernel<<<1, kThreads, 0, st>>>(partials, blocks, out_norm);
     return launched("mz_tensor_table_global_norm");
 }
@@ -350,7 +364,7 @@ int mz_tensor_table_clip(void* stream, const mz_tensor_table_t* table, const voi
     if (!blocks) {
         norm_finish_kernel<<<1, kThreads, 0, st>>>(partials, 0, out_norm);
     } else {
-        norm_partials_kernel<<<blocks, kThreads, 0, st>>>(in_memory(table, device_table), partials);
+        launch_partials(in_memory(table, device_table), blocks, table->large, st, partials);
         clip_kernel<<<blocks, kThreads, 0, st>>>(in_memory(table, device_table), partials, blocks, max_norm, out_norm);
     }
     return launched("mz_tensor_table_clip");

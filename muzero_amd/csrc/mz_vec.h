@@ -32,6 +32,13 @@ template <typename T, int V>
 __device__ inline Vec<T, V> load(const T* p) {
     return *reinterpret_cast<const Vec<T, V>*>(p);
 }
+// 16 bytes that are not read again soon: they need not displace what the caches hold
+template <typename T, int V>
+__device__ inline Vec<T, V> load_streaming(const T* p) {
+    static_assert(sizeof(T) * V == 16, "a whole access");
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+    return __builtin_bit_cast(Vec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const Words*>(p)));
+}
 template <typename T, int V>
 struct __attribute__((packed, aligned(sizeof(T)))) Elements {
     T v[V];
