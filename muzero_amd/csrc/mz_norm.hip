@@ -9,10 +9,18 @@ using mz_norm::kSplitThreads;
 using mz_norm::Norm;
 using mz_norm::Plan;
 
-int vector_of(const mz_group_norm_t* c) {          // the widest access of at most 16 bytes that stays within a group
-    int v = 16 / mz::dtype_size(c->dtype);
-    while ((c->channels / c->groups) % v) v >>= 1;
-    return v;
+// The widest vectors of at most 16 bytes.  A group of V channels or more is cut into such vectors, its last one moved back to
+// end with it; smaller groups stand side by side in a vector where the channels are a multiple of it, else in one of two
+// channels or none.
+void choose_vector(const mz_group_norm_t* c, int* v, int* q) {
+    const int most = 16 / mz::dtype_size(c->dtype), d = c->channels / c->groups;
+    *q = 1;
+    *v = most;
+    if (d >= most) return;
+    if ((d & (d - 1)) == 0 && c->channels % most == 0) *q = most / d;
+    else if (d == 1 && c->channels % 2 == 0) *v = *q = 2;
+    else
+        while (*v > d) *v >>= 1;
 }
 
 int check(const mz_group_norm_t* c) {
@@ -35,26 +43,26 @@ int log2_up(long v) {
 
 // Lanes of a workgroup of `threads`, and the vectors a thread then holds of a tile.
 int lay_out(Norm& d, int v, int item, int threads) {
-    const int dv = d.D / v, lth = log2_up(threads);
+    const int dv = (d.U + v - 1) / v, lth = log2_up(threads), units = d.C / d.U;
     d.pieces = 1;
     d.samples = 1;
     d.ldv = log2_up(dv);
-    if (d.ldv > lth) {                              // a group wider than the workgroup: pieces of it
+    if (d.ldv > lth) {                              // a unit wider than the workgroup: pieces of it
         d.ldv = lth;
         d.pieces = (dv + threads - 1) / threads;
         d.lgs = d.lrows = 0;
         d.gs = 1;
-        d.tiles = d.G * d.pieces;
+        d.tiles = units * d.pieces;
         return 0;
     }
-    const int all = log2_up(d.G), room = lth - d.ldv;
-    const long line = (128 + (long)d.D * item - 1) / ((long)d.D * item);
+    const int all = log2_up(units), room = lth - d.ldv;
+    const long line = (128 + (long)d.U * item - 1) / ((long)d.U * item);
     d.lgs = log2_up(line) < all ? log2_up(line) : all;
     if (d.lgs > room) d.lgs = room;
     while (d.lgs < all && d.lgs < room && (threads >> (d.ldv + d.lgs)) > d.S) ++d.lgs;     // more lanes than positions
-    d.tiles = (d.G + (1 << d.lgs) - 1) >> d.lgs;
-    d.gs = (d.G + d.tiles - 1) / d.tiles;           // tiles of even size
-    d.tiles = (d.G + d.gs - 1) / d.gs;
+    d.tiles = (units + (1 << d.lgs) - 1) >> d.lgs;
+    d.gs = (units + d.tiles - 1) / d.tiles;         // tiles of even size
+    d.tiles = (units + d.gs - 1) / d.gs;
     d.lrows = lth - d.ldv - d.lgs;
     const int ls = log2_up(d.S);
     if (ls < d.lrows) {                             // small samples: several side by side
@@ -83,7 +91,9 @@ Plan plan(const mz_group_norm_t* c) {
         d.rs[i] = c->residual_strides[i];
         d.ds[i] = c->dy_strides[i];
     }
-    const int v = vector_of(c), item = mz::dtype_size(c->dtype);
+    choose_vector(c, &p.v, &p.q);
+    d.U = p.q > 1 ? p.v : d.D;
+    const int v = p.v, item = mz::dtype_size(c->dtype);
     // the smallest workgroup whose registers hold a tile, one wavefront without barriers if it may be
     for (const int threads : {64, 256, 512}) {
         const int k = lay_out(d, v, item, threads);
@@ -126,10 +136,10 @@ int launched(const char* what) {
     return MZ_OK;
 }
 
-void run(int dtype, const Plan& p, int v, bool backward, hipStream_t st) {
-    if (dtype == MZ_F32) backward ? mz_norm::backward<float>(p, v, st) : mz_norm::forward<float>(p, v, st);
-    else if (dtype == MZ_F16) backward ? mz_norm::backward<mz::f16>(p, v, st) : mz_norm::forward<mz::f16>(p, v, st);
-    else backward ? mz_norm::backward<mz::bf16>(p, v, st) : mz_norm::forward<mz::bf16>(p, v, st);
+void run(int dtype, const Plan& p, bool backward, hipStream_t st) {
+    if (dtype == MZ_F32) backward ? mz_norm::backward<float>(p, st) : mz_norm::forward<float>(p, st);
+    else if (dtype == MZ_F16) backward ? mz_norm::backward<mz::f16>(p, st) : mz_norm::forward<mz::f16>(p, st);
+    else backward ? mz_norm::backward<mz::bf16>(p, st) : mz_norm::forward<mz::bf16>(p, st);
 }
 
 }  // namespace
@@ -161,7 +171,7 @@ int mz_group_norm_forward(void* stream, const mz_group_norm_t* c, const void* x,
     d.mean = out_mean;
     d.rstd = out_rstd;
     d.ws = static_cast<float*>(workspace);
-    run(c->dtype, p, vector_of(c), false, static_cast<hipStream_t>(stream));
+    run(c->dtype, p, false, static_cast<hipStream_t>(stream));
     return launched("mz_group_norm_forward");
 }
 
@@ -188,7 +198,7 @@ int mz_group_norm_backward(void* stream, const mz_group_norm_t* c, const void* x
     d.dw = out_dweight;
     d.db = out_dbias;
     d.ws = static_cast<float*>(workspace);
-    run(c->dtype, p, vector_of(c), true, static_cast<hipStream_t>(stream));
+    run(c->dtype, p, true, static_cast<hipStream_t>(stream));
     return launched("mz_group_norm_backward");
 }
 

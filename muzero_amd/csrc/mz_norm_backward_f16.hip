@@ -1,0 +1,6 @@
+// The backward kernels of group norm (mz_norm_dev.h) for f16 states.
+#include "mz_norm_dev.h"
+
+namespace mz_norm {
+template void backward<mz::f16>(const Plan&, hipStream_t);
+}  // namespace mz_norm

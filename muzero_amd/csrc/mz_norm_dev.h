@@ -8,10 +8,13 @@
 // dresidual); 10 to 40 operations a value.
 //
 // A workgroup takes a tile of a sample: whole groups side by side, at least a 128-byte line of channels where there are as
-// many.  A thread keeps one vector of V channels (V divides D: one group a vector) and walks down the positions, so
-// consecutive lanes read consecutive addresses.  Vectors of a group and groups of a tile are padded to powers of two over
-// the lanes: a lane's group, vector and position come from bits of its number, and a group's sum is a butterfly over the
-// other bits (group_sum), without index tables or divisions.  Two ways through:
+// many.  A thread keeps one vector of V channels and walks down the positions, so consecutive lanes read consecutive
+// addresses.  Vectors are as wide as an access can be (16 bytes) whatever D is: where D is no multiple of V, a group's last
+// vector is moved back to end with the group, and its first `dup` channels, which are the vector's before it too, count
+// nothing in the group's sums (they are stored twice, alike); where D is smaller than V, a vector holds Q = V / D groups with
+// a sum of its own each.  "Units" are what lanes share: a group, or the Q groups of a vector.  Vectors of a unit and units of
+// a tile are padded to powers of two over the lanes: a lane's unit, vector and position come from bits of its number, and a
+// unit's sums are a butterfly over the other bits (group_sum), without index tables or divisions.  Two ways through:
 //   resident  the tile's values stay in registers between the statistics and the result: one launch, every input read once.
 //   split     samples too large for that (K vectors a thread do not hold the tile): positions are cut into chunks over
 //             several workgroups; a first launch leaves each chunk's partial sums, a second adds them up and reads again.
@@ -31,12 +34,12 @@ constexpr int kMostSplits = 64;
 
 struct Norm {
     long N, S;
-    int C, G, D, act, params_f32;
+    int C, G, D, U, act, params_f32;          // U: channels of a unit
     float eps;
     long xs[2], rs[2], ds[2];
-    // lanes: bits [vector in group : ldv][group in tile : lgs][position : lrows][sample : the rest]
+    // lanes: bits [vector in unit : ldv][unit in tile : lgs][position : lrows][sample : the rest]
     int ldv, lgs, lrows, samples;
-    int gs, tiles, pieces;                    // groups of a tile, tiles of a sample, pieces of a group wider than a workgroup
+    int gs, tiles, pieces;                    // units of a tile, tiles of a sample, pieces of a unit wider than a workgroup
     int splits;                               // chunks of positions of a sample (split)
     long chunk, blocks;                       // positions of a chunk; workgroups of a tile (resident backward)
     const void *x, *res, *w, *b, *dy;
@@ -46,13 +49,14 @@ struct Norm {
 
 struct Plan {
     Norm d;
+    int v, q;                                 // channels of a vector, groups of it
     int threads, k;                           // of the resident kernels; k = 0: split
 };
 
 struct Lane {
-    int vec, group, row, sample;              // vector of its group, group of its tile, first position, sample
-    int dv;                                   // vectors of the group (of this piece)
-    int g, ch;                                // group and first channel within the sample
+    int vec, unit, row, sample;               // vector of its unit, unit of its tile, first position, sample
+    int g, ch, dup;                           // unit and first channel within the sample, channels that are another lane's too
+    int first, width;                         // this piece's first channel within its unit, and channels
     bool live;                                // not padding
 };
 
@@ -61,26 +65,29 @@ __device__ Lane lane_of(const Norm& d, int tile) {
     Lane l;
     const int t = threadIdx.x;
     l.vec = t & ((1 << d.ldv) - 1);
-    l.group = (t >> d.ldv) & ((1 << d.lgs) - 1);
+    l.unit = (t >> d.ldv) & ((1 << d.lgs) - 1);
     l.row = (t >> (d.ldv + d.lgs)) & ((1 << d.lrows) - 1);
     l.sample = t >> (d.ldv + d.lgs + d.lrows);
-    l.dv = d.D / V;
-    int first = 0, gs = d.gs;
+    int gs = d.gs;
+    l.first = 0;
+    l.width = d.U;
     if (d.pieces > 1) {
         l.g = tile / d.pieces;
-        first = (tile - l.g * d.pieces) << d.ldv;
-        l.dv = l.dv - first < 1 << d.ldv ? l.dv - first : 1 << d.ldv;
+        l.first = ((tile - l.g * d.pieces) << d.ldv) * V;
+        l.width = d.U - l.first < V << d.ldv ? d.U - l.first : V << d.ldv;
     } else {
         l.g = tile * d.gs;
-        gs = d.G - l.g < gs ? d.G - l.g : gs;
+        gs = d.C / d.U - l.g < gs ? d.C / d.U - l.g : gs;
     }
-    l.live = l.vec < l.dv && l.group < gs && l.sample < d.samples;
-    if (l.group < gs) l.g += l.group;         // padding reads what a live lane reads, and counts nothing
-    l.ch = l.g * d.D + (first + (l.live ? l.vec : 0)) * V;
+    l.live = l.vec * V < l.width && l.unit < gs && l.sample < d.samples;
+    if (l.unit < gs) l.g += l.unit;           // padding reads what a live lane reads, and counts nothing
+    const int in_unit = l.first + (l.live ? l.vec * V : 0), from = in_unit < d.U - V ? in_unit : d.U - V;
+    l.dup = in_unit - from;
+    l.ch = l.g * d.U + from;
     return l;
 }
 
-// Sums of N values over the lanes of a group (all its vectors and positions, of one sample), to every lane of it.
+// Sums of N values over the lanes of a unit (all its vectors and positions, of one sample), to every lane of it.
 // `scratch`: TH * N floats that no thread still reads; an alternation of two needs no barrier in between.
 template <int TH, int N>
 __device__ inline void group_sum(float (&v)[N], const Norm& d, float* scratch) {
@@ -92,8 +99,8 @@ __device__ inline void group_sum(float (&v)[N], const Norm& d, float* scratch) {
 #pragma unroll
         for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m);
     if (TH == 64) return;
-    const int t = threadIdx.x, groups = (pitch - 1) & ~(dvp - 1) & ~63;       // bits of the wavefront's number that are a group's
-    // one slot for each group of a wavefront
+    const int t = threadIdx.x, groups = (pitch - 1) & ~(dvp - 1) & ~63;       // bits of the wavefront's number that are a unit's
+    // one slot for each unit of a wavefront
     const int slot = (t & 63 & (pitch - 1)) >> (d.ldv < 6 ? d.ldv : 6);
 #pragma unroll
     for (int k = 0; k < N; ++k) scratch[(t >> 6) * 64 * N + slot * N + k] = v[k];      // lanes of one slot hold the same value
@@ -144,6 +151,13 @@ template <typename T, int V>
 __device__ inline void load_params(const Norm& d, int c, float (&w)[V], float (&b)[V]) {
     load_param<T, V>(d.w, d.params_f32, c, 1.f, w);
     load_param<T, V>(d.b, d.params_f32, c, 0.f, b);
+}
+
+template <int Q>
+__device__ inline void load_stats(const Norm& d, long at, float (&mu)[Q], float (&rs)[Q]) {
+    const Vec<float, Q> m = mz::load<float, Q>(d.mean + at), r = mz::load<float, Q>(d.rstd + at);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) mu[q] = m[q], rs[q] = r[q];
 }
 
 // No activation and relu share their code: a floor below which z is cut, and a threshold that z has to be above for its slope.
@@ -205,12 +219,28 @@ __device__ inline void with_activation(int act, F f) {       // the choice is ou
     else f(Cut(act));
 }
 
-template <typename T, int V, typename A>
-__device__ inline void apply(const Vec<T, V>& x, const Vec<T, V>* res, float mu, float rs, const float (&w)[V], const float (&b)[V],
-                             const A& act, T* y) {
+// sums over a vector's channels of f(value), for each of its Q groups
+template <int Q, typename T, int V, typename F>
+__device__ inline void sum_up(const Vec<T, V>& x, int dup, bool counts, F f, float (&sum)[Q]) {
+    float p[Q] = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i * Q / V] = f(x[i], i * Q / V, p[i * Q / V]);
+    if (Q == 1 && dup) {                                    // once more without the other lane's
+        p[0] = 0.f;
+#pragma unroll
+        for (int i = 1; i < V; ++i)
+            if (i >= dup) p[0] = f(x[i], 0, p[0]);
+    }
+#pragma unroll
+    for (int j = 0; j < Q; ++j) sum[j] += counts ? p[j] : 0.f;
+}
+
+template <int Q, typename T, int V, typename A>
+__device__ inline void apply(const Vec<T, V>& x, const Vec<T, V>* res, const float (&mu)[Q], const float (&rs)[Q], const float (&w)[V],
+                             const float (&b)[V], const A& act, T* y) {
     float f[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = fmaf((x[i] - mu) * rs, w[i], b[i]);
+    for (int i = 0; i < V; ++i) f[i] = fmaf((x[i] - mu[i * Q / V]) * rs[i * Q / V], w[i], b[i]);
     if (res)
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] += (*res)[i];
@@ -220,13 +250,13 @@ __device__ inline void apply(const Vec<T, V>& x, const Vec<T, V>* res, float mu,
 }
 
 // h and dz of V values
-template <typename T, int V, typename A>
-__device__ inline void back_values(const Vec<T, V>& x, const Vec<T, V>& dy, const Vec<T, V>* res, float mu, float rs, const float (&w)[V],
-                                   const float (&b)[V], const A& act, float (&h)[V], float (&dz)[V]) {
+template <int Q, typename T, int V, typename A>
+__device__ inline void back_values(const Vec<T, V>& x, const Vec<T, V>& dy, const Vec<T, V>* res, const float (&mu)[Q], const float (&rs)[Q],
+                                   const float (&w)[V], const float (&b)[V], const A& act, float (&h)[V], float (&dz)[V]) {
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        h[i] = (x[i] - mu) * rs;
+        h[i] = (x[i] - mu[i * Q / V]) * rs[i * Q / V];
         z[i] = fmaf(h[i], w[i], b[i]);
     }
     if (res)
@@ -235,14 +265,26 @@ __device__ inline void back_values(const Vec<T, V>& x, const Vec<T, V>& dy, cons
 #pragma unroll
     for (int i = 0; i < V; ++i) dz[i] = dy[i] * act.slope(z[i]);
 }
-template <typename T, int V>
-__device__ inline void back_store(const Norm& d, long base, unsigned at, float rs, float a, float q, const float (&w)[V], const float (&h)[V],
-                                  float (&dz)[V]) {
+template <int Q, typename T, int V>
+__device__ inline void back_store(const Norm& d, long base, unsigned at, const float (&rs)[Q], const float (&aq)[2 * Q], const float (&w)[V],
+                                  const float (&h)[V], float (&dz)[V], const T*) {
     if (d.dres) mz::store<T, V>(static_cast<T*>(d.dres) + base + at, dz);
     if (d.dx) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) dz[i] = rs * (fmaf(dz[i], w[i], -a) - h[i] * q);
+        for (int i = 0; i < V; ++i) dz[i] = rs[i * Q / V] * (fmaf(dz[i], w[i], -aq[i * Q / V]) - h[i] * aq[Q + i * Q / V]);
         mz::store<T, V>(static_cast<T*>(d.dx) + base + at, dz);
+    }
+}
+
+// dz, dz h into the channels' sums and, times the weight (0 for another lane's channels), into the groups' sums
+template <int Q, int V>
+__device__ inline void back_sum(const float (&h)[V], const float (&dz)[V], const float (&wq)[V], float (&s1)[V], float (&s2)[V], float (&aq)[2 * Q]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        s1[i] += dz[i];
+        s2[i] = fmaf(dz[i], h[i], s2[i]);
+        aq[i * Q / V] = fmaf(dz[i], wq[i], aq[i * Q / V]);
+        aq[Q + i * Q / V] = fmaf(dz[i] * wq[i], h[i], aq[Q + i * Q / V]);
     }
 }
 
@@ -276,9 +318,9 @@ __device__ inline void forget(Vec<T, V> (&v)[K]) {
             }
 }
 
-template <typename T, int V, int TH, int K>
+template <typename T, int V, int Q, int TH, int K>
 __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
-    __shared__ float scratch[2][TH];
+    __shared__ float scratch[2][TH == 64 ? 1 : TH * Q];
     const int S = (int)d.S, step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
     for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y)
@@ -292,32 +334,26 @@ __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
             if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
             float w[V], b[V];
             load_params<T, V>(d, l.ch, w, b);
-            float sum[1] = {0.f};
+            float sum[Q] = {}, mu[Q], rs[Q];
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (k * step < S) {
-                    float p = 0.f;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) p += xv[k][i];
-                    sum[0] += live && l.row + k * step < S ? p : 0.f;
-                }
+                if (k * step < S)
+                    sum_up<Q>(xv[k], l.dup, live && l.row + k * step < S, [](float v, int, float p) { return p + v; }, sum);
             group_sum<TH>(sum, d, scratch[0]);
-            const float mu = sum[0] * inv;
-            sum[0] = 0.f;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) mu[q] = sum[q] * inv, sum[q] = 0.f;
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (k * step < S) {
-                    float p = 0.f;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) p = fmaf(xv[k][i] - mu, xv[k][i] - mu, p);
-                    sum[0] += live && l.row + k * step < S ? p : 0.f;
-                }
+                if (k * step < S)
+                    sum_up<Q>(xv[k], l.dup, live && l.row + k * step < S,
+                              [&](float v, int q, float p) { return fmaf(v - mu[q], v - mu[q], p); }, sum);
             group_sum<TH>(sum, d, scratch[1]);
-            const float rs = 1.f / sqrtf(sum[0] * inv + d.eps);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) rs[q] = 1.f / sqrtf(sum[q] * inv + d.eps);
             if (!live) continue;
             if (d.mean && l.vec == 0 && l.row == 0) {
-                d.mean[(n0 + j) * d.G + l.g] = mu;
-                d.rstd[(n0 + j) * d.G + l.g] = rs;
+                mz::store<float, Q>(d.mean + (n0 + j) * d.G + l.g * Q, mu);
+                mz::store<float, Q>(d.rstd + (n0 + j) * d.G + l.g * Q, rs);
             }
             T* y = static_cast<T*>(d.y) + n0 * d.S * d.C;
             const int at = (j * S + l.row) * d.C + l.ch;
@@ -325,24 +361,26 @@ __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
                     if (l.row + k * step < S)
-                        apply<T, V>(xv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, y + (unsigned)(at + k * step * d.C));
+                        apply<Q>(xv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, y + (unsigned)(at + k * step * d.C));
             });
         }
 }
 
 // A workgroup keeps its tile and strides over the samples: the channels' sums for dweight and dbias stay in registers and
 // leave one row of ws [blocks][2][C] a workgroup.
-template <typename T, int V, int TH, int K>
+template <typename T, int V, int Q, int TH, int K>
 __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
-    __shared__ float scratch[TH == 64 ? 1 : TH * (V > 2 ? 2 * V : 4)];
+    __shared__ float scratch[TH == 64 ? 1 : TH * (2 * V > 4 * Q ? 2 * V : 4 * Q)];
     const int S = (int)d.S, step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
     const long block = blockIdx.x;
     int turn = 0;
     for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y) {
         const Lane l = lane_of<V>(d, tile);
-        float w[V], b[V], s1[V] = {}, s2[V] = {};
+        float w[V], b[V], wq[V], s1[V] = {}, s2[V] = {};
         load_params<T, V>(d, l.ch, w, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) wq[i] = Q == 1 && i < l.dup ? 0.f : w[i];
         for (long n0 = block * d.samples; n0 < d.N; n0 += d.blocks * d.samples, turn ^= 1) {
             const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;
             const bool live = l.live && l.sample < left;
@@ -351,25 +389,20 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
             load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
             load_rows<T, V, K>(gv, static_cast<const T*>(d.dy) + n0 * d.ds[0], j * (int)d.ds[0] + l.ch, (int)d.ds[1], l.row, step, S);
             if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
-            const float mu = d.mean[(n0 + j) * d.G + l.g], rs = d.rstd[(n0 + j) * d.G + l.g];
-            float aq[2] = {0.f, 0.f};
+            float mu[Q], rs[Q], aq[2 * Q] = {};
+            load_stats(d, (n0 + j) * d.G + l.g * Q, mu, rs);
             with_activation(d.act, [&](auto act) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     if (!live || l.row + k * step >= S) continue;
                     float h[V], dz[V];
-                    back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        s1[i] += dz[i];
-                        s2[i] = fmaf(dz[i], h[i], s2[i]);
-                        aq[0] = fmaf(dz[i], w[i], aq[0]);
-                        aq[1] = fmaf(dz[i] * w[i], h[i], aq[1]);
-                    }
+                    back_values<Q>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
+                    back_sum<Q>(h, dz, wq, s1, s2, aq);
                 }
             });
-            group_sum<TH>(aq, d, TH == 64 ? scratch : scratch + turn * 2 * TH);
-            const float a = aq[0] * inv, q = aq[1] * inv;
+            group_sum<TH>(aq, d, TH == 64 ? scratch : scratch + turn * 2 * Q * TH);
+#pragma unroll
+            for (int q = 0; q < 2 * Q; ++q) aq[q] *= inv;
             const long out = n0 * d.S * d.C;
             const int at = (j * S + l.row) * d.C + l.ch;
             forget(xv);
@@ -380,15 +413,15 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
                 for (int k = 0; k < K; ++k) {
                     if (!live || l.row + k * step >= S) continue;
                     float h[V], dz[V];
-                    back_values<T, V>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
-                    back_store<T, V>(d, out, (unsigned)(at + k * step * d.C), rs, a, q, w, h, dz);
+                    back_values<Q>(xv[k], gv[k], d.res ? &rv[k] : nullptr, mu, rs, w, b, act, h, dz);
+                    back_store<Q>(d, out, (unsigned)(at + k * step * d.C), rs, aq, w, h, dz, (const T*)nullptr);
                 }
             });
         }
         if (!d.dw && !d.db) continue;
         column_sum<TH>(s1, d, scratch);
         column_sum<TH>(s2, d, TH == 64 ? scratch : scratch + TH * V);
-        if (TH > 64) __syncthreads();                           // before another tile's sums
+        if (TH > 64) __syncthreads();                       // before another tile's sums
         if (l.live && l.row == 0 && l.sample == 0) {
             mz::store<float, V>(d.ws + block * 2 * d.C + l.ch, s1);
             mz::store<float, V>(d.ws + block * 2 * d.C + d.C + l.ch, s2);
@@ -411,9 +444,9 @@ __device__ inline void for_each_part(const Norm& d, F f) {
             f(Part{n, s0, s0 + d.chunk < d.S ? s0 + d.chunk : d.S, (int)blockIdx.x, tile});
         }
 }
-// where (split, piece) of a group stands among its splits * pieces partial results
+// where (split, piece) of a unit stands among its splits * pieces partial results
 __device__ inline long part_at(const Norm& d, const Part& p, const Lane& l) {
-    return ((p.n * d.G + l.g) * d.splits + p.split) * d.pieces + (d.pieces > 1 ? p.tile % d.pieces : 0);
+    return ((p.n * (d.C / d.U) + l.g) * d.splits + p.split) * d.pieces + (d.pieces > 1 ? p.tile % d.pieces : 0);
 }
 
 constexpr int kBatch = 4;                       // vectors of a thread under way at once
@@ -425,89 +458,100 @@ __device__ inline void load_batch(Vec<T, V> (&v)[kBatch], const T* p, long strid
     for (int k = 0; k < kBatch; ++k) v[k] = mz::load<T, V>(p + (s + k * step < end ? s + k * step : s) * stride);
 }
 
-// ws [N][G][splits][pieces][2]: mean and sum of squared deviations of each part
-template <typename T, int V>
+// ws [N][units][splits][pieces][2][Q]: mean and sum of squared deviations of each part
+template <typename T, int V, int Q>
 __global__ void __launch_bounds__(kSplitThreads) norm_stats_kernel(Norm d) {
-    __shared__ float scratch[2][kSplitThreads];
+    __shared__ float scratch[2][kSplitThreads * Q];
     const int step = 1 << d.lrows;
     for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
-        float count = 0.f, mean = 0.f, m2 = 0.f;
+        float count = 0.f, mean[Q] = {}, m2[Q] = {};
         if (l.live) {
             const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
             for (long s = p.s0 + l.row; s < p.s1; s += kBatch * step) {     // a batch on its own, then merged
                 Vec<T, V> v[kBatch];
                 load_batch(v, x, d.xs[1], s, step, p.s1);
-                float sum = 0.f, more = 0.f, dev = 0.f;
+                float sum[Q] = {}, more = 0.f, m[Q], dev[Q] = {};
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
-                    float q = 0.f;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) q += v[k][i];
-                    const bool in = s + k * step < p.s1;
-                    sum += in ? q : 0.f;
-                    more += in ? (float)V : 0.f;
+                    sum_up<Q>(v[k], l.dup, s + k * step < p.s1, [](float v, int, float p) { return p + v; }, sum);
+                    more += s + k * step < p.s1 ? (float)(Q == 1 ? V - l.dup : V / Q) : 0.f;
                 }
-                const float m = sum / more;
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    float q = 0.f;
+                for (int q = 0; q < Q; ++q) m[q] = sum[q] / more;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) q = fmaf(v[k][i] - m, v[k][i] - m, q);
-                    dev += s + k * step < p.s1 ? q : 0.f;
+                for (int k = 0; k < kBatch; ++k)
+                    sum_up<Q>(v[k], l.dup, s + k * step < p.s1, [&](float v, int q, float p) { return fmaf(v - m[q], v - m[q], p); }, dev);
+                const float f = more / (count + more);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    const float e = m[q] - mean[q];
+                    mean[q] = fmaf(e, f, mean[q]);
+                    m2[q] += dev[q] + e * e * count * f;
                 }
-                const float e = m - mean, f = more / (count + more);
-                mean = fmaf(e, f, mean);
-                m2 += dev + e * e * count * f;
                 count += more;
             }
         }
-        const float all = (float)(p.s1 - p.s0) * (float)(l.dv * V);
-        float v[1] = {count * mean};
+        const float all = (float)(p.s1 - p.s0) * (float)(Q == 1 ? l.width : V / Q);
+        float v[Q], mu[Q];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) v[q] = count * mean[q];
         group_sum<kSplitThreads>(v, d, scratch[0]);
-        const float mu = v[0] / all;
-        v[0] = count > 0.f ? fmaf(count * (mean - mu), mean - mu, m2) : 0.f;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            mu[q] = v[q] / all;
+            v[q] = count > 0.f ? fmaf(count * (mean[q] - mu[q]), mean[q] - mu[q], m2[q]) : 0.f;
+        }
         group_sum<kSplitThreads>(v, d, scratch[1]);
         if (l.live && l.vec == 0 && l.row == 0) {
-            float* ws = d.ws + 2 * part_at(d, p, l);
-            ws[0] = mu;
-            ws[1] = v[0];
+            float* ws = d.ws + 2 * Q * part_at(d, p, l);
+            mz::store<float, Q>(ws, mu);
+            mz::store<float, Q>(ws + Q, v);
         }
     });
 }
 
-template <typename T, int V>
+template <typename T, int V, int Q>
 __global__ void __launch_bounds__(kSplitThreads) norm_apply_kernel(Norm d) {
-    __shared__ float scratch[2][kSplitThreads];
+    __shared__ float scratch[2][kSplitThreads * Q];
     const int step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
     for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
-        const long ng = p.n * d.G + l.g;
         const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
         const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
-        // the group's parts, over its lanes (a part's share of the values: its positions times its vectors)
-        const float* ws = d.ws + 2 * ng * d.splits * d.pieces;
+        // the unit's parts, over its lanes (a part's share of the values: its positions times its channels)
         const int parts = d.splits * d.pieces, lanes = 1 << (d.ldv + d.lrows), mine = (l.row << d.ldv) + l.vec;
+        const float* ws = d.ws + 2 * Q * (p.n * (d.C / d.U) + l.g) * parts;
         const auto count = [&](int e) {
-            const int split = d.pieces > 1 ? e / d.pieces : e, piece = e - split * d.pieces, left = d.D / V - (piece << d.ldv);
+            const int split = d.pieces > 1 ? e / d.pieces : e, from = ((e - split * d.pieces) << d.ldv) * V;
             const long positions = split * d.chunk + d.chunk < d.S ? d.chunk : d.S - split * d.chunk;
-            return (float)positions * (float)((left < 1 << d.ldv ? left : 1 << d.ldv) * V);
+            const int channels = Q > 1 ? V / Q : d.U - from < V << d.ldv ? d.U - from : V << d.ldv;
+            return (float)positions * (float)channels;
         };
-        float a[1] = {0.f};
-        if (l.group < d.gs)
-            for (int e = mine; e < parts; e += lanes) a[0] = fmaf(count(e), ws[2 * e], a[0]);
+        float a[Q] = {}, mu[Q], rs[Q];
+        if (l.unit < d.gs)
+            for (int e = mine; e < parts; e += lanes) {
+                const Vec<float, Q> m = mz::load<float, Q>(ws + 2 * Q * e);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) a[q] = fmaf(count(e), m[q], a[q]);
+            }
         group_sum<kSplitThreads>(a, d, scratch[0]);
-        const float mu = a[0] * inv;
-        a[0] = 0.f;
-        if (l.group < d.gs)
-            for (int e = mine; e < parts; e += lanes) a[0] += fmaf(count(e) * (ws[2 * e] - mu), ws[2 * e] - mu, ws[2 * e + 1]);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) mu[q] = a[q] * inv, a[q] = 0.f;
+        if (l.unit < d.gs)
+            for (int e = mine; e < parts; e += lanes) {
+                const Vec<float, Q> m = mz::load<float, Q>(ws + 2 * Q * e), m2 = mz::load<float, Q>(ws + 2 * Q * e + Q);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) a[q] += fmaf(count(e) * (m[q] - mu[q]), m[q] - mu[q], m2[q]);
+            }
         group_sum<kSplitThreads>(a, d, scratch[1]);
-        const float rs = 1.f / sqrtf(a[0] * inv + d.eps);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) rs[q] = 1.f / sqrtf(a[q] * inv + d.eps);
         if (!l.live) return;
         if (d.mean && p.split == 0 && l.vec == 0 && l.row == 0 && (d.pieces == 1 || p.tile % d.pieces == 0)) {
-            d.mean[ng] = mu;
-            d.rstd[ng] = rs;
+            mz::store<float, Q>(d.mean + p.n * d.G + l.g * Q, mu);
+            mz::store<float, Q>(d.rstd + p.n * d.G + l.g * Q, rs);
         }
         float w[V], b[V];
         load_params<T, V>(d, l.ch, w, b);
@@ -519,25 +563,27 @@ __global__ void __launch_bounds__(kSplitThreads) norm_apply_kernel(Norm d) {
                 if (res) load_batch(r, res, d.rs[1], s, step, p.s1);
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k)
-                    if (s + k * step < p.s1) apply<T, V>(v[k], res ? &r[k] : nullptr, mu, rs, w, b, act, y + (s + k * step) * d.C);
+                    if (s + k * step < p.s1) apply<Q>(v[k], res ? &r[k] : nullptr, mu, rs, w, b, act, y + (s + k * step) * d.C);
             }
         });
     });
 }
 
 // ws: sums of dz and dz h of a chunk's positions, [N * splits][2][C], then sums of dz w and dz w h of each part,
-// [N][G][splits][pieces][2]
-template <typename T, int V>
+// [N][units][splits][pieces][2][Q]
+template <typename T, int V, int Q>
 __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
-    __shared__ float scratch[2][kSplitThreads * (V > 2 ? V : 2)];
+    __shared__ float scratch[2][kSplitThreads * (V > 2 * Q ? V : 2 * Q)];
     const int step = 1 << d.lrows;
     for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
-        const long ng = p.n * d.G + l.g;
-        float s1[V] = {}, s2[V] = {}, w[V], b[V];
+        float s1[V] = {}, s2[V] = {}, w[V], b[V], wq[V], aq[2 * Q] = {};
         load_params<T, V>(d, l.ch, w, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) wq[i] = Q == 1 && i < l.dup ? 0.f : w[i];
         if (l.live) {
-            const float mu = d.mean[ng], rs = d.rstd[ng];
+            float mu[Q], rs[Q];
+            load_stats(d, p.n * d.G + l.g * Q, mu, rs);
             const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
             const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
             const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
@@ -551,7 +597,7 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
                     for (int k = 0; k < kBatch; ++k) {
                         if (s + k * step >= p.s1) continue;
                         float h[V], dz[V];
-                        back_values<T, V>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
+                        back_values<Q>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
 #pragma unroll
                         for (int i = 0; i < V; ++i) {
                             s1[i] += dz[i];
@@ -561,11 +607,10 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
                 }
             });
         }
-        float aq[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            aq[0] = fmaf(s1[i], w[i], aq[0]);
-            aq[1] = fmaf(s2[i], w[i], aq[1]);
+            aq[i * Q / V] = fmaf(s1[i], wq[i], aq[i * Q / V]);
+            aq[Q + i * Q / V] = fmaf(s2[i], wq[i], aq[Q + i * Q / V]);
         }
         __syncthreads();
         group_sum<kSplitThreads>(aq, d, scratch[0]);
@@ -575,38 +620,37 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
             float* ws = d.ws + (p.n * d.splits + p.split) * 2 * d.C + l.ch;
             mz::store<float, V>(ws, s1);
             mz::store<float, V>(ws + d.C, s2);
-            if (l.vec == 0) {
-                float* at = d.ws + d.N * d.splits * 2 * d.C + 2 * part_at(d, p, l);
-                at[0] = aq[0];
-                at[1] = aq[1];
-            }
+            if (l.vec == 0) mz::store<float, 2 * Q>(d.ws + d.N * d.splits * 2 * d.C + 2 * Q * part_at(d, p, l), aq);
         }
     });
 }
 
-template <typename T, int V>
+template <typename T, int V, int Q>
 __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) {
-    __shared__ float scratch[2][2 * kSplitThreads];
+    __shared__ float scratch[2][2 * Q * kSplitThreads];
     const int step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
     int turn = 0;
     for_each_part(d, [&](const Part& p) {
         const Lane l = lane_of<V>(d, p.tile);
-        const long ng = p.n * d.G + l.g;
         const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
         const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
         const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
-        const float* ws = d.ws + d.N * d.splits * 2 * d.C + 2 * ng * d.splits * d.pieces;
-        float aq[2] = {0.f, 0.f};
-        if (l.group < d.gs)
-            for (int e = (l.row << d.ldv) + l.vec; e < d.splits * d.pieces; e += 1 << (d.ldv + d.lrows)) {
-                aq[0] += ws[2 * e];
-                aq[1] += ws[2 * e + 1];
+        const int parts = d.splits * d.pieces;
+        const float* ws = d.ws + d.N * d.splits * 2 * d.C + 2 * Q * (p.n * (d.C / d.U) + l.g) * parts;
+        float aq[2 * Q] = {}, mu[Q], rs[Q];
+        if (l.unit < d.gs)
+            for (int e = (l.row << d.ldv) + l.vec; e < parts; e += 1 << (d.ldv + d.lrows)) {
+                const Vec<float, 2 * Q> part = mz::load<float, 2 * Q>(ws + 2 * Q * e);
+#pragma unroll
+                for (int q = 0; q < 2 * Q; ++q) aq[q] += part[q];
             }
         group_sum<kSplitThreads>(aq, d, scratch[turn]);
         turn ^= 1;
         if (!l.live) return;
-        const float mu = d.mean[ng], rs = d.rstd[ng], a = aq[0] * inv, q = aq[1] * inv;
+#pragma unroll
+        for (int q = 0; q < 2 * Q; ++q) aq[q] *= inv;
+        load_stats(d, p.n * d.G + l.g * Q, mu, rs);
         float w[V], b[V];
         load_params<T, V>(d, l.ch, w, b);
         const long out = p.n * d.S * d.C + l.ch;
@@ -620,8 +664,8 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
                 for (int k = 0; k < kBatch; ++k) {
                     if (s + k * step >= p.s1) continue;
                     float h[V], dz[V];
-                    back_values<T, V>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
-                    back_store<T, V>(d, out + (s + k * step) * d.C, 0, rs, a, q, w, h, dz);
+                    back_values<Q>(v[k], g[k], res ? &r[k] : nullptr, mu, rs, w, b, act, h, dz);
+                    back_store<Q>(d, out + (s + k * step) * d.C, 0, rs, aq, w, h, dz, (const T*)nullptr);
                 }
             }
         });
@@ -666,12 +710,15 @@ template <int V>
 using Int = std::integral_constant<int, V>;
 
 template <typename T, typename F>
-void with_vector(int v, F f) {
-    if constexpr (sizeof(T) == 2)
-        if (v == 8) return f(Int<8>{});
-    if (v == 4) f(Int<4>{});
-    else if (v == 2) f(Int<2>{});
-    else f(Int<1>{});
+void with_vector(int v, int q, F f) {
+    if constexpr (sizeof(T) == 2) {
+        if (v == 8) return q == 8 ? f(Int<8>{}, Int<8>{}) : q == 4 ? f(Int<8>{}, Int<4>{}) : q == 2 ? f(Int<8>{}, Int<2>{}) : f(Int<8>{}, Int<1>{});
+        if (v == 4) return f(Int<4>{}, Int<1>{});
+    } else {
+        if (v == 4) return q == 4 ? f(Int<4>{}, Int<4>{}) : q == 2 ? f(Int<4>{}, Int<2>{}) : f(Int<4>{}, Int<1>{});
+    }
+    if (v == 2) return q == 2 ? f(Int<2>{}, Int<2>{}) : f(Int<2>{}, Int<1>{});
+    f(Int<1>{}, Int<1>{});
 }
 template <typename F>
 void with_size(const Plan& p, F f) {                // threads, and vectors a thread, of the resident kernels
@@ -688,46 +735,46 @@ void with_size(const Plan& p, F f) {                // threads, and vectors a th
 inline unsigned grid_of(long total) { return (unsigned)(total < (1L << 22) ? total : 1L << 22); }
 
 template <typename T>
-void forward(const Plan& p, int v, hipStream_t st) {
+void forward(const Plan& p, hipStream_t st) {
     const Norm& d = p.d;
-    with_vector<T>(v, [&](auto v_) {
-        constexpr int V = v_.value;
+    with_vector<T>(p.v, p.q, [&](auto v, auto q) {
+        constexpr int V = v.value, Q = q.value;
         if (p.k) {
             const dim3 grid(grid_of((d.N + d.samples - 1) / d.samples), d.tiles < 65535 ? d.tiles : 65535);
-            with_size(p, [&](auto th, auto k) { norm_forward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
+            with_size(p, [&](auto th, auto k) { norm_forward_kernel<T, V, Q, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
         } else {
             const dim3 grid(d.splits, d.tiles < 65535 ? d.tiles : 65535, d.N < 65535 ? d.N : 65535);
-            norm_stats_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
-            norm_apply_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
+            norm_stats_kernel<T, V, Q><<<grid, kSplitThreads, 0, st>>>(d);
+            norm_apply_kernel<T, V, Q><<<grid, kSplitThreads, 0, st>>>(d);
         }
     });
 }
 
 template <typename T>
-void backward(const Plan& p, int v, hipStream_t st) {
+void backward(const Plan& p, hipStream_t st) {
     const Norm& d = p.d;
     const bool empty = d.N == 0 || d.S == 0;
     if (!empty)
-        with_vector<T>(v, [&](auto v_) {
-            constexpr int V = v_.value;
+        with_vector<T>(p.v, p.q, [&](auto v, auto q) {
+            constexpr int V = v.value, Q = q.value;
             if (p.k) {
                 const dim3 grid((unsigned)d.blocks, d.tiles < 65535 ? d.tiles : 65535);
-                with_size(p, [&](auto th, auto k) { norm_backward_kernel<T, V, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
+                with_size(p, [&](auto th, auto k) { norm_backward_kernel<T, V, Q, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
             } else {
                 const dim3 grid(d.splits, d.tiles < 65535 ? d.tiles : 65535, d.N < 65535 ? d.N : 65535);
-                norm_back_sums_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
-                if (d.dx || d.dres) norm_back_apply_kernel<T, V><<<grid, kSplitThreads, 0, st>>>(d);
+                norm_back_sums_kernel<T, V, Q><<<grid, kSplitThreads, 0, st>>>(d);
+                if (d.dx || d.dres) norm_back_apply_kernel<T, V, Q><<<grid, kSplitThreads, 0, st>>>(d);
             }
         });
     if (d.dw || d.db)           // of no rows: zeros
         norm_params_kernel<T><<<(2 * d.C + 15) / 16, 1024, 0, st>>>(d, empty ? 0 : p.k ? d.blocks : d.N * d.splits);
 }
 
-extern template void forward<float>(const Plan&, int, hipStream_t);
-extern template void forward<mz::f16>(const Plan&, int, hipStream_t);
-extern template void forward<mz::bf16>(const Plan&, int, hipStream_t);
-extern template void backward<float>(const Plan&, int, hipStream_t);
-extern template void backward<mz::f16>(const Plan&, int, hipStream_t);
-extern template void backward<mz::bf16>(const Plan&, int, hipStream_t);
+extern template void forward<float>(const Plan&, hipStream_t);
+extern template void forward<mz::f16>(const Plan&, hipStream_t);
+extern template void forward<mz::bf16>(const Plan&, hipStream_t);
+extern template void backward<float>(const Plan&, hipStream_t);
+extern template void backward<mz::f16>(const Plan&, hipStream_t);
+extern template void backward<mz::bf16>(const Plan&, hipStream_t);
 
 }  // namespace mz_norm

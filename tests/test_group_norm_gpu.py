@@ -29,6 +29,19 @@ CASES = [
     (2, (101,), 520, 40, F32, None, True, 'f32'), (3, (37,), 1030, 103, BF16, 'silu', False, 'f32'),
 ]
 
+# groups smaller than an access, of odd sizes, and wider than a workgroup, in registers and split over positions
+CASES += [
+    (33, (3, 3), 64, 32, BF16, 'relu', True, 'f32'), (5, (4,), 64, 64, F16, 'silu', True, 'f32'), (5, (4,), 24, 12, BF16, 'gelu', False, 'f32'),
+    (7, (6,), 20, 10, BF16, 'tanh', True, 'same'), (7, (6,), 12, 4, F16, 'relu', True, 'f32'), (3, (5, 5), 36, 4, BF16, 'silu', True, 'f32'),
+    (3, (5,), 100, 4, F16, None, False, 'f32'), (2, (70,), 44, 4, F32, 'gelu', True, 'f32'), (2, (7,), 35, 7, BF16, 'relu', False, 'f32'),
+    (2, (9,), 6, 6, F32, 'tanh', True, 'f32'), (3, (), 4099, 1, BF16, 'relu', True, 'f32'), (1, (50, 50), 27, 3, F16, 'silu', True, 'f32'),
+    (2, (2500,), 16, 16, BF16, 'relu', True, 'f32'), (2, (2500,), 16, 4, F16, 'gelu', False, 'f32'), (2, (2500,), 16, 8, BF16, None, True, 'same'),
+    (2, (1500,), 20, 5, F32, 'relu', True, 'f32'), (3, (1500,), 6, 2, F32, 'silu', False, 'f32'), (2, (1400,), 8, 8, F32, 'tanh', True, 'f32'),
+    (1, (33,), 8197, 1, F16, 'gelu', True, 'f32'), (4, (361,), 64, 32, BF16, 'relu', True, 'f32'), (4, (361,), 64, 64, F32, 'silu', True, 'f32'),
+    (3, (2304,), 64, 32, BF16, 'relu', True, 'f32'), (129, (2,), 9, 1, F32, 'relu', True, 'f32'), (1000, (), 15, 3, BF16, 'silu', False, 'f32'),
+    (2, (400,), 130, 1, BF16, 'relu', True, 'f32'), (2, (90,), 7, 1, F16, 'gelu', True, None), (3, (129,), 1026, 2, F32, 'relu', False, 'f32'),
+]
+
 
 def make(case, seed=0):
     N, shape, C, G, dtype, activation, residual, params = case
