@@ -55,21 +55,28 @@ int lay_out(Norm& d, int v, int item, int threads) {
         d.tiles = units * d.pieces;
         return 0;
     }
-    const int all = log2_up(units), room = lth - d.ldv;
-    const long line = (128 + (long)d.U * item - 1) / ((long)d.U * item);
-    d.lgs = log2_up(line) < all ? log2_up(line) : all;
-    if (d.lgs > room) d.lgs = room;
-    while (d.lgs < all && d.lgs < room && (threads >> (d.ldv + d.lgs)) > d.S) ++d.lgs;     // more lanes than positions
+    // Units of a tile: those of a 128-byte line, or more where that leaves fewer lanes idle over the positions, the padding of
+    // the tiles and the samples side by side -- unless there are too few tiles to begin with, or a thread would then hold more
+    // vectors than the kernels that read ahead do (nine positions on eight rows of lanes: two vectors a thread, nine sixteenths
+    // of them live; on four rows three, three quarters: backward of 34722 x 9 x 128 f32 in groups of 4 148 -> 116 us).
+    const int all = log2_up(units), room = lth - d.ldv, most = all < room ? all : room;
+    const int line = log2_up((128 + (long)d.U * item - 1) / ((long)d.U * item)), least = line < most ? line : most, ls = log2_up(d.S);
+    double best = INFINITY;
+    long k = 0;
+    for (int lgs = least; lgs <= most; ++lgs) {
+        const int tiles = (units + (1 << lgs) - 1) >> lgs, lrows = lth - d.ldv - lgs < ls ? lth - d.ldv - lgs : ls;
+        const long steps = (d.S + (1L << lrows) - 1) >> lrows;
+        const double cost = (double)tiles * (double)steps / (double)(1 << (lth - d.ldv - lgs - lrows));
+        if (lgs > least && (cost >= best || steps > 4 || d.N * tiles < 2048)) continue;
+        best = cost;
+        k = steps;
+        d.lgs = lgs;
+        d.lrows = lrows;
+    }
+    d.samples = 1 << (lth - d.ldv - d.lgs - d.lrows);
     d.tiles = (units + (1 << d.lgs) - 1) >> d.lgs;
     d.gs = (units + d.tiles - 1) / d.tiles;         // tiles of even size
     d.tiles = (units + d.gs - 1) / d.gs;
-    d.lrows = lth - d.ldv - d.lgs;
-    const int ls = log2_up(d.S);
-    if (ls < d.lrows) {                             // small samples: several side by side
-        d.samples = 1 << (d.lrows - ls);
-        d.lrows = ls;
-    }
-    const long k = (d.S + (1L << d.lrows) - 1) >> d.lrows;
     return k < 1 << 20 ? (int)k : 1 << 20;
 }
 
@@ -106,6 +113,9 @@ Plan plan(const mz_group_norm_t* c) {
         p.k = k;
         const long sets = (d.N + d.samples - 1) / d.samples, fill = 2048 / (threads / 64) / d.tiles;
         d.blocks = sets < fill ? sets : fill > 1 ? fill : 1;                   // eight wavefronts a CU
+        // twenty wavefronts a CU, which read ahead; 312500 x 128 bf16: 44 us, with a wavefront a set of samples 60
+        const long ahead = 5120 / d.tiles;
+        d.forward_blocks = threads > 64 || k > 2 || sets < ahead ? sets : ahead > 1 ? ahead : 1;
         d.splits = 1;
         return p;
     }

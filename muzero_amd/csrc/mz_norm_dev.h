@@ -41,7 +41,7 @@ struct Norm {
     int ldv, lgs, lrows, samples;
     int gs, tiles, pieces;                    // units of a tile, tiles of a sample, pieces of a unit wider than a workgroup
     int splits;                               // chunks of positions of a sample (split)
-    long chunk, blocks;                       // positions of a chunk; workgroups of a tile (resident backward)
+    long chunk, forward_blocks, blocks;       // positions of a chunk; workgroups of a tile (resident, forward and backward)
     const void *x, *res, *w, *b, *dy;
     void *y, *dx, *dres, *dw, *db;
     float *mean, *rstd, *ws;
@@ -366,6 +366,71 @@ __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
         }
 }
 
+// What a thread reads of one set of samples
+template <typename T, int V, int K, int ARRAYS>
+struct Held {
+    Vec<T, V> v[ARRAYS][K];
+};
+
+// The same for wavefronts on their own with one or two vectors a thread: they stride over the samples and read the next set
+// while they work on one, as too little of theirs would be under way otherwise.
+template <typename T, int V, int Q, int K>
+__global__ void __launch_bounds__(64) norm_forward_ahead_kernel(Norm d) {
+    const int S = (int)d.S, step = 1 << d.lrows;
+    const float inv = 1.f / ((float)d.S * (float)d.D);
+    for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y) {
+        const Lane l = lane_of<V>(d, tile);
+        const auto left = [&](long n0) { return d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples; };      // samples of a set
+        const auto load = [&](Held<T, V, K, 2>& h, long n0) {
+            const int j = l.live && l.sample < left(n0) ? l.sample : 0;
+            load_rows<T, V, K>(h.v[0], static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
+            if (d.res) load_rows<T, V, K>(h.v[1], static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
+        };
+        const long stride = (long)gridDim.x * d.samples;
+        Held<T, V, K, 2> held, next;
+        long n0 = (long)blockIdx.x * d.samples;
+        if (n0 < d.N) load(held, n0);
+        float w[V], b[V];
+        load_params<T, V>(d, l.ch, w, b);
+        for (; n0 < d.N; n0 += stride) {
+            if (n0 + stride < d.N) load(next, n0 + stride);
+            const bool live = l.live && l.sample < left(n0);
+            const int j = live ? l.sample : 0;
+            float sum[Q] = {}, mu[Q], rs[Q];
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k * step < S)
+                    sum_up<Q>(held.v[0][k], l.dup, live && l.row + k * step < S, [](float v, int, float p) { return p + v; }, sum);
+            group_sum<64>(sum, d, nullptr);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) mu[q] = sum[q] * inv, sum[q] = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k * step < S)
+                    sum_up<Q>(held.v[0][k], l.dup, live && l.row + k * step < S,
+                              [&](float v, int q, float p) { return fmaf(v - mu[q], v - mu[q], p); }, sum);
+            group_sum<64>(sum, d, nullptr);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) rs[q] = 1.f / sqrtf(sum[q] * inv + d.eps);
+            if (live) {
+                if (d.mean && l.vec == 0 && l.row == 0) {
+                    mz::store<float, Q>(d.mean + (n0 + j) * d.G + l.g * Q, mu);
+                    mz::store<float, Q>(d.rstd + (n0 + j) * d.G + l.g * Q, rs);
+                }
+                T* y = static_cast<T*>(d.y) + n0 * d.S * d.C;
+                const int at = (j * S + l.row) * d.C + l.ch;
+                with_activation(d.act, [&](auto act) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k)
+                        if (l.row + k * step < S)
+                            apply<Q>(held.v[0][k], d.res ? &held.v[1][k] : nullptr, mu, rs, w, b, act, y + (unsigned)(at + k * step * d.C));
+                });
+            }
+            held = next;
+        }
+    }
+}
+
 // A workgroup keeps its tile and strides over the samples: the channels' sums for dweight and dbias stay in registers and
 // leave one row of ws [blocks][2][C] a workgroup.
 template <typename T, int V, int Q, int TH, int K>
@@ -381,14 +446,24 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
         load_params<T, V>(d, l.ch, w, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) wq[i] = Q == 1 && i < l.dup ? 0.f : w[i];
-        for (long n0 = block * d.samples; n0 < d.N; n0 += d.blocks * d.samples, turn ^= 1) {
-            const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;
-            const bool live = l.live && l.sample < left;
+        const auto left = [&](long n0) { return d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples; };      // samples of a set
+        const auto load = [&](Held<T, V, K, 3>& h, long n0) {
+            const int j = l.live && l.sample < left(n0) ? l.sample : 0;
+            load_rows<T, V, K>(h.v[0], static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
+            load_rows<T, V, K>(h.v[1], static_cast<const T*>(d.dy) + n0 * d.ds[0], j * (int)d.ds[0] + l.ch, (int)d.ds[1], l.row, step, S);
+            if (d.res) load_rows<T, V, K>(h.v[2], static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
+        };
+        constexpr bool AHEAD = TH == 64 && K <= 4;          // the next set is read while one is worked on
+        const long stride = d.blocks * d.samples;
+        Held<T, V, K, 3> held, next;
+        long n0 = block * d.samples;
+        if (AHEAD && n0 < d.N) load(held, n0);
+        for (; n0 < d.N; n0 += stride, turn ^= 1) {
+            if (!AHEAD) load(held, n0);
+            else if (n0 + stride < d.N) load(next, n0 + stride);
+            const bool live = l.live && l.sample < left(n0);
             const int j = live ? l.sample : 0;
-            Vec<T, V> xv[K], gv[K], rv[K];
-            load_rows<T, V, K>(xv, static_cast<const T*>(d.x) + n0 * d.xs[0], j * (int)d.xs[0] + l.ch, (int)d.xs[1], l.row, step, S);
-            load_rows<T, V, K>(gv, static_cast<const T*>(d.dy) + n0 * d.ds[0], j * (int)d.ds[0] + l.ch, (int)d.ds[1], l.row, step, S);
-            if (d.res) load_rows<T, V, K>(rv, static_cast<const T*>(d.res) + n0 * d.rs[0], j * (int)d.rs[0] + l.ch, (int)d.rs[1], l.row, step, S);
+            auto &xv = held.v[0], &gv = held.v[1], &rv = held.v[2];
             float mu[Q], rs[Q], aq[2 * Q] = {};
             load_stats(d, (n0 + j) * d.G + l.g * Q, mu, rs);
             with_activation(d.act, [&](auto act) {
@@ -417,6 +492,7 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
                     back_store<Q>(d, out, (unsigned)(at + k * step * d.C), rs, aq, w, h, dz, (const T*)nullptr);
                 }
             });
+            if (AHEAD) held = next;
         }
         if (!d.dw && !d.db) continue;
         column_sum<TH>(s1, d, scratch);
@@ -674,27 +750,25 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
 
 // ---- dweight, dbias ---------------------------------------------------------------------------------------------------
 
-// ws [rows][2][C] summed over its rows: 16 columns a workgroup, 64 rows side by side, in 64 bits (sums over every position
+// ws [rows][2][C] summed over its rows: 8 columns a workgroup, 128 rows side by side, in 64 bits (sums over every position
 // of a batch, which may cancel)
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_params_kernel(Norm d, long rows) {
-    __shared__ double part[1024];
-    const int t = threadIdx.x, c = blockIdx.x * 16 + (t & 15);
+    __shared__ double part[16][8];
+    const int t = threadIdx.x, c = blockIdx.x * 8 + (t & 7), column = c < 2 * d.C ? c : 2 * d.C - 1;
     double s = 0.0;
-    if (c < 2 * d.C)
-        for (long r = t >> 4; r < rows; r += 4 * 64) {
-            float v[4];
+    for (long r = t >> 3; r < rows; r += 8 * 128) {
+        float v[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = r + k * 64 < rows ? d.ws[(r + k * 64) * 2 * d.C + c] : 0.f;
+        for (int k = 0; k < 8; ++k) v[k] = d.ws[(r + k * 128 < rows ? r + k * 128 : r) * 2 * d.C + column];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s += v[k];
-        }
-    s += __shfl_xor(s, 16);
-    s += __shfl_xor(s, 32);
-    part[t] = s;
+        for (int k = 0; k < 8; ++k) s += r + k * 128 < rows ? v[k] : 0.f;
+    }
+    for (int m = 8; m < 64; m <<= 1) s += __shfl_xor(s, m);
+    if ((t & 63) < 8) part[t >> 6][t & 7] = s;
     __syncthreads();
-    if (t < 16 && c < 2 * d.C) {
-        for (int j = 1; j < 16; ++j) s += part[j * 64 + t];
+    if (t < 8 && c < 2 * d.C) {
+        for (int j = 1; j < 16; ++j) s += part[j][t];
         const bool which = c >= d.C;
         void* out = which ? d.dw : d.db;
         const int at = which ? c - d.C : c;
@@ -740,8 +814,11 @@ void forward(const Plan& p, hipStream_t st) {
     with_vector<T>(p.v, p.q, [&](auto v, auto q) {
         constexpr int V = v.value, Q = q.value;
         if (p.k) {
-            const dim3 grid(grid_of((d.N + d.samples - 1) / d.samples), d.tiles < 65535 ? d.tiles : 65535);
-            with_size(p, [&](auto th, auto k) { norm_forward_kernel<T, V, Q, th.value, k.value><<<grid, th.value, 0, st>>>(d); });
+            const dim3 grid(grid_of(d.forward_blocks), d.tiles < 65535 ? d.tiles : 65535);
+            with_size(p, [&](auto th, auto k) {
+                if constexpr (th.value == 64 && k.value == 2) norm_forward_ahead_kernel<T, V, Q, 2><<<grid, 64, 0, st>>>(d);
+                else norm_forward_kernel<T, V, Q, th.value, k.value><<<grid, th.value, 0, st>>>(d);
+            });
         } else {
             const dim3 grid(d.splits, d.tiles < 65535 ? d.tiles : 65535, d.N < 65535 ? d.N : 65535);
             norm_stats_kernel<T, V, Q><<<grid, kSplitThreads, 0, st>>>(d);
@@ -767,7 +844,7 @@ void backward(const Plan& p, hipStream_t st) {
             }
         });
     if (d.dw || d.db)           // of no rows: zeros
-        norm_params_kernel<T><<<(2 * d.C + 15) / 16, 1024, 0, st>>>(d, empty ? 0 : p.k ? d.blocks : d.N * d.splits);
+        norm_params_kernel<T><<<(2 * d.C + 7) / 8, 1024, 0, st>>>(d, empty ? 0 : p.k ? d.blocks : d.N * d.splits);
 }
 
 extern template void forward<float>(const Plan&, hipStream_t);
