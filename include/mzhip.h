@@ -506,7 +506,7 @@ int mz_replay_targets(void* stream, const mz_replay_config_t* config, const int3
  * What a training step on the replay targets consists of besides its products.  The reference leaves these to Keras
  * (training.py:13-51,157-204).  All calls enqueue on `stream` (which belongs to the current device), allocate nothing,
  * keep nothing between calls and may be captured into a graph; a workspace belongs to one call at a time.  Pointers to
- * elements are aligned to one element, no further.  Sums and statistics are held in 32 bits or more. */
+ * elements are aligned to one element, no further; a workspace of the norm calls to 4 bytes, of the others to 8.  Sums and statistics are held in 32 bits or more. */
 typedef enum mz_dtype { MZ_F32 = 0, MZ_F16 = 1, MZ_BF16 = 2 } mz_dtype;
 typedef enum mz_activation { MZ_ACT_NONE = 0, MZ_ACT_RELU = 1, MZ_ACT_SILU = 2, MZ_ACT_GELU = 3 /* by erf */,
                              MZ_ACT_TANH = 4 } mz_activation;

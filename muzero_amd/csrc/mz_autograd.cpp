@@ -7,9 +7,11 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstring>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/mzhip.h"
@@ -67,34 +69,50 @@ struct On {
     explicit On(const c10::Device& d) : guard(d), stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(d.index()).stream()) {}
 };
 
-// A leaf's gradient is accumulated on the stream its accumulation node was made on, and the node lives as long as any
-// autograd graph that holds it.  A backward pass captured while such a graph of another stream lives would leave the
-// capture, which ends the process: refused before anything is captured.
-void refuse_live_leaves(const c10::Device& d, std::initializer_list<const Tensor*> tensors) {
-    if (!done(mz_stream_is_capturing(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(d.index()).stream()))) return;
-    const c10::Stream current = c10::impl::VirtualGuardImpl(d.type()).getStream(d);
-    for (const Tensor* t : tensors) {
-        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (!node) continue;
+// A backward pass runs every node of the graph on the stream the node was made on; a leaf's accumulation node lives as long
+// as any graph that holds it.  A backward pass captured while the captured graph reaches a node of a stream outside the
+// capture -- through a leaf that an eager graph holds, or an eager graph in front -- would leave the capture, which ends the
+// process: refused when the forward pass is captured, before anything is launched.
+void refuse_nodes_outside_capture(const c10::Device& d, std::initializer_list<const Tensor*> inputs) {
+    const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(d.index());
+    if (!done(mz_stream_is_capturing(here.stream()))) return;
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    const auto visit = [&](std::shared_ptr<torch::autograd::Node> node) {
+        if (node && seen.insert(node.get()).second) todo.push_back(std::move(node));
+    };
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->requires_grad()) visit(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        const auto node = std::move(todo.back());
+        todo.pop_back();
         const auto made_on = node->stream();
-        if (made_on && *made_on != current)
-            refuse("this forward pass is being captured while an autograd graph of the same leaf tensor from another stream is "
-                   "alive: delete its outputs (the loss among them) before capturing");
+        if (made_on && *made_on != here.unwrap() &&
+            !done(mz_stream_is_capturing(c10::hip::HIPStreamMasqueradingAsCUDA(*made_on).stream())))
+            refuse("this forward pass is being captured, and its backward pass would reach a node (", node->name(), ") of a stream outside "
+                   "the capture: an eager autograd graph of the same leaf tensors is alive, or lies in front of this call; delete its "
+                   "outputs (the loss among them), or detach the input, before capturing");
+        for (const auto& edge : node->next_edges()) visit(edge.function);
     }
 }
 
-// Differentiable once: under create_graph the gradients pass through a node that refuses to be differentiated.
+// Differentiable once: under create_graph the gradients pass through a node that depends on all they were computed from and
+// refuses to be differentiated.
 struct Once : torch::autograd::Function<Once> {
-    static Tensor forward(AutogradContext*, const Tensor& gradient, const Tensor&) { return gradient.view_as(gradient); }
+    static Tensor forward(AutogradContext*, const Tensor& gradient, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                          const OptTensor&) {
+        return gradient.view_as(gradient);
+    }
     static variable_list backward(AutogradContext*, variable_list) {
         throw std::runtime_error("muzero_amd's training operators are differentiable once");
     }
 };
-variable_list once(variable_list gradients, const Tensor& from) {
-    if (at::GradMode::is_enabled())
+variable_list once(variable_list gradients, const std::array<Tensor, 5>& from) {
+    if (at::GradMode::is_enabled()) {
+        const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
         for (Tensor& g : gradients)
-            if (g.defined()) g = Once::apply(g, from);
+            if (g.defined()) g = Once::apply(g, opt(from[0]), opt(from[1]), opt(from[2]), opt(from[3]), opt(from[4]));
+    }
     return gradients;
 }
 
@@ -182,7 +200,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
                                         mean + config.batch * config.groups, data(dy), data(dx), data(dresidual), data(dweight),
                                         data(dbias), data(ws), bytes));
         }
-        return once({dx, dweight, dbias, dresidual, Tensor()}, x);
+        return once({dx, dweight, dbias, dresidual, Tensor()}, {x, weight, bias, residual, dys[0]});
     }
 };
 
@@ -229,7 +247,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, cons
     c.config.eps = eps;
     const bool differentiable = at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias) || wants_grad(residual));
     if (differentiable)
-        refuse_live_leaves(x.device(), {&x, weight ? &*weight : &x, bias ? &*bias : &x, residual ? &*residual : &x});
+        refuse_nodes_outside_capture(x.device(), {&x, weight ? &*weight : &x, bias ? &*bias : &x, residual ? &*residual : &x});
     {
         const at::NoGradGuard off;
         c.x = states(x, c.config.x_strides);
@@ -358,14 +376,14 @@ struct CategoricalLoss : torch::autograd::Function<CategoricalLoss> {
         c.position = saved[3];
         c.weights = saved[4];
         const Tensor grad = loss_run(c, false, true, dloss[0]).second;
-        return once({grad, Tensor()}, c.logits);
+        return once({grad, Tensor()}, {c.logits, dloss[0]});
     }
 };
 
 Tensor categorical_loss(const Tensor& logits, const Tensor& targets, const OptTensor& game, const OptTensor& position, const OptTensor& weights) {
     LossCall c = describe(logits, targets, game, position, weights);
     if (!at::GradMode::is_enabled() || !logits.requires_grad()) return loss_run(c, true, false, Tensor()).first;
-    refuse_live_leaves(logits.device(), {&logits});
+    refuse_nodes_outside_capture(logits.device(), {&logits});
     return CategoricalLoss::apply(logits, &c);
 }
 
@@ -422,6 +440,11 @@ struct TensorList {
             }
         }
         require_hip(device);
+    }
+    void check_unmoved() const {
+        for (size_t i = 0; i < tensors.size(); ++i)
+            if (tensors[i].data_ptr() != described[i].data || (!outputs.empty() && out[i].data_ptr() != outputs[i]))
+                refuse("tensor ", i, " or its output has other memory than when the set was made");
     }
     const std::vector<Tensor>& written() const { return outputs.empty() ? tensors : out; }
     void* const* output_table() const { return outputs.empty() ? nullptr : outputs.data(); }
@@ -487,6 +510,7 @@ class GradientSet {
         memory_ = host.to(list_.device);
     }
     Tensor global_norm() const {
+        list_.check_unmoved();
         void* const table = this->table();
         return list_.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
             return mz_tensor_table_global_norm(stream, &table_, table, ws, bytes, norm);
@@ -495,6 +519,7 @@ class GradientSet {
     Tensor clip_by_global_norm(double max_norm) const {
         list_.check_clip(max_norm);
         if (!overlap_.empty()) refuse("cannot clip: ", overlap_);
+        list_.check_unmoved();
         void* const table = this->table();
         const Tensor norm = list_.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
             return mz_tensor_table_clip(stream, &table_, table, max_norm, ws, bytes, norm);

@@ -179,6 +179,7 @@ int check(int32_t n, const mz_tensor_t* tensors, Total* total) {
 int check_workspace(void* workspace, int64_t bytes, const float* out_norm) {
     MZ_REQUIRE(workspace && bytes >= MZ_GLOBAL_NORM_WORKSPACE, "workspace of %lld bytes, %d needed", (long long)bytes, MZ_GLOBAL_NORM_WORKSPACE);
     MZ_REQUIRE(out_norm, "out_norm is NULL");
+    MZ_REQUIRE(mz::aligned(sizeof(double), {workspace}) && mz::aligned(sizeof(float), {out_norm}), "workspace or out_norm is not aligned");
     return MZ_OK;
 }
 

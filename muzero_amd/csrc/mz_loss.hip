@@ -172,6 +172,9 @@ extern "C" int mz_categorical_loss(void* stream, const mz_categorical_t* c, cons
     if (c->unroll == 0 || c->batch == 0) return MZ_OK;
     MZ_REQUIRE(c->batch <= int64_t(1) << 31 && c->unroll <= int64_t(1) << 31, "more than 2^31 rows of a step, or steps");
     MZ_REQUIRE(logits && (targets || c->target_positions * c->target_games == 0), "logits/targets is NULL");
+    MZ_REQUIRE(mz::aligned(mz::dtype_size(c->dtype), {logits, out_dlogits}) && mz::aligned(sizeof(float), {targets, weights, dloss, out_loss}) &&
+                   (c->index_bytes == 0 || mz::aligned(c->index_bytes, {game, position})),
+               "an array is not aligned to its type");
     if (!out_loss && !out_dlogits) return MZ_OK;
     Loss d = {};
     d.U = c->unroll;

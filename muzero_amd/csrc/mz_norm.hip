@@ -172,6 +172,9 @@ int mz_group_norm_forward(void* stream, const mz_group_norm_t* c, const void* x,
     Plan p = plan(c);
     const int64_t need = workspace_of(p, false);
     MZ_REQUIRE(workspace_bytes >= need && (workspace || !need), "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    MZ_REQUIRE(mz::aligned(mz::dtype_size(c->dtype), {x, residual, out_y}) && mz::aligned(mz::dtype_size(c->param_dtype), {weight, bias}) &&
+                   mz::aligned(sizeof(float), {out_mean, out_rstd, workspace}),
+               "an array is not aligned to its type");
     Norm& d = p.d;
     d.x = x;
     d.res = residual;
@@ -195,6 +198,10 @@ int mz_group_norm_backward(void* stream, const mz_group_norm_t* c, const void* x
     const bool empty = c->batch == 0 || c->positions == 0;
     MZ_REQUIRE(empty || (x && mean && rstd && dy), "x/mean/rstd/dy is NULL");
     MZ_REQUIRE(workspace_bytes >= need && (workspace || !need), "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    MZ_REQUIRE(mz::aligned(mz::dtype_size(c->dtype), {x, residual, dy, out_dx, out_dresidual}) &&
+                   mz::aligned(mz::dtype_size(c->param_dtype), {weight, bias, out_dweight, out_dbias}) &&
+                   mz::aligned(sizeof(float), {mean, rstd, workspace}),
+               "an array is not aligned to its type");
     Norm& d = p.d;
     d.x = x;
     d.res = residual;

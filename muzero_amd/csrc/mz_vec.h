@@ -2,6 +2,7 @@
 #pragma once
 #include "mz_common.h"
 #include <cstdint>
+#include <initializer_list>
 #include <type_traits>
 
 namespace mz {
@@ -10,6 +11,12 @@ typedef _Float16 f16;
 typedef __bf16 bf16;
 
 inline int dtype_size(int dtype) { return dtype == MZ_F32 ? 4 : dtype == MZ_F16 || dtype == MZ_BF16 ? 2 : 0; }
+
+inline bool aligned(size_t bytes, std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if ((uintptr_t)p % bytes) return false;
+    return true;
+}
 
 // V elements that are loaded and stored as one access, kept as they lie in memory: 16-bit elements stay two to a register
 // until they are used.  Aligned like ONE element: gfx950 takes a 4-, 8- or 16-byte access at any element address, so rows of

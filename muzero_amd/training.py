@@ -56,7 +56,8 @@ class GradientSet:
     tensors: 1 to 8192 float32, float16 and bfloat16 tensors of one device, each dense in some order of its dimensions.
     out: the tensors that clipping writes, of the same shapes, strides and types; None = the tensors themselves.  The set
     keeps the tensors alive, and has to be kept as long as a graph with calls of it is replayed; it is made outside
-    captures.  Results are ordered on the current stream; a set may be used on several streams at once."""
+    captures.  A tensor that was given other memory since is refused.  Results are ordered on the current stream; a set may be
+    used on several streams at once."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None) -> None:
         self._set = _list(_lib.native().GradientSet, list(tensors), None if out is None else list(out))

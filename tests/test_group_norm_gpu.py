@@ -269,3 +269,58 @@ def test_capture_beside_a_living_eager_graph_is_refused():
     torch.cuda.synchronize()
     want, off = oracle(x, 4, w, None, None, None).backward(rows(x))
     check('dweight', g, want['dweight'], off['dweight'], F32)
+
+
+@pytest.mark.parametrize('which', range(4))
+def test_second_derivatives_are_refused_whatever_requires_grad(which):
+    from muzero_amd.layers import group_norm
+    x, G, w, b, activation, res, dy = make((2, (9,), 16, 4, F32, 'silu', True, 'f32'))
+    part = [t.clone().requires_grad_(k == which) for k, t in enumerate((x, w, b, res))]
+    up = dy.clone().requires_grad_()
+    y = group_norm(part[0], G, part[1], part[2], activation=activation, residual=part[3])
+    (g,) = torch.autograd.grad(y, part[which], up, create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        g.sum().backward()
+
+
+def test_the_same_tensor_as_state_residual_and_both_parameters():
+    from muzero_amd.layers import group_norm
+    x, G, w, _, _, _, dy = make((3, (9,), 32, 8, F32, 'gelu', False, 'f32'))
+    leaf, p = x.clone().requires_grad_(), w.clone().requires_grad_()
+    got = torch.autograd.grad(group_norm(leaf, G, p, p, activation='gelu', residual=leaf), [leaf, p], dy)
+    want, off = oracle(x, G, w, w, 'gelu', x).backward(rows(dy))
+    check('dx', got[0], want['dx'] + want['dresidual'], off['dx'] + off['dresidual'] + 2 * HALF[F32] * (np.abs(want['dx']) + np.abs(want['dresidual'])), F32)
+    check('dw', got[1], want['dweight'] + want['dbias'], off['dweight'] + off['dbias'] + 2 * HALF[F32] * (np.abs(want['dweight']) + np.abs(want['dbias'])), F32)
+
+
+def test_backward_beyond_2_to_the_31_elements():
+    from muzero_amd.layers import group_norm
+    N, S, C = 70000, 961, 32
+    x = torch.zeros(N, S, C, dtype=F16, device='cuda')
+    x[-1] = torch.randn(S, C, device='cuda').to(F16)
+    leaf = x.requires_grad_()
+    w = torch.ones(C, device='cuda', requires_grad=True)
+    y = group_norm(leaf, 4, w)
+    dy = torch.zeros(1, 1, 1, dtype=F16, device='cuda').expand(N, S, C)          # a gradient in the last sample alone, strides 0 before
+    up = torch.zeros_like(y)
+    up[-1] = torch.randn(S, C, device='cuda').to(F16)
+    assert torch.autograd.grad(y, leaf, dy, retain_graph=True)[0].count_nonzero() == 0
+    gx, gw = torch.autograd.grad(y, [leaf, w], up)
+    want, off = oracle(x[-1:].detach(), 4, torch.ones(C), None, None, None).backward(rows(up[-1:]))
+    check('dx', gx[-1:], want['dx'], off['dx'], F16)
+    check('dweight', gw, want['dweight'], off['dweight'], F32)
+    assert gx[:-1].count_nonzero() == 0
+
+
+def test_capture_is_refused_through_the_graph_in_front_as_well():
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.layers import group_norm
+    x, p = torch.randn(2, 9, 16, device='cuda'), torch.ones(16, device='cuda', requires_grad=True)
+    eager = x * p                                           # holds p's accumulation node, and is a node itself
+    with pytest.raises(MuZeroError, match='outside the capture'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            group_norm(x * p, 4)
+    with pytest.raises(MuZeroError, match='outside the capture'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            group_norm(eager, 4)
+    assert torch.isfinite(group_norm(eager, 4)).all()

@@ -198,3 +198,25 @@ def test_tensor_tables_are_checked_where_they_are_built():
     assert lib.mz_tensor_table_global_norm(None, None, 0x100, *args) == -1
     assert lib.mz_tensor_table_global_norm(None, ctypes.byref(info), 0x100, 0x100, L.MZ_GLOBAL_NORM_WORKSPACE - 1, 0x100) == -1
     assert lib.mz_tensor_table_global_norm(None, ctypes.byref(info), 0x100, 0x100, L.MZ_GLOBAL_NORM_WORKSPACE, None) == -1
+
+
+def test_c_entries_refuse_arrays_that_are_not_aligned_to_their_type():
+    L, lib = _lib()
+    A, ws = 0x100000, L.MZ_GLOBAL_NORM_WORKSPACE
+    norm = L.GroupNorm(batch=2, positions=3, channels=8, groups=2, dtype=2, param_dtype=0, activation=1, eps=1e-5)
+    good = [A, A, A, A, A, A, A, A]                                    # x, residual, weight, bias, y, mean, rstd, workspace
+    for i, off in ((0, 1), (1, 1), (2, 2), (3, 2), (4, 1), (5, 2), (6, 2), (7, 2)):
+        args = list(good)
+        args[i] += off
+        assert lib.mz_group_norm_forward(None, ctypes.byref(norm), *args, 1 << 20) == -1, i
+    for i, off in enumerate((1, 1, 2, 2, 2, 2, 1, 1, 1, 2, 2, 2)):     # x, residual, weight, bias, mean, rstd, dy, dx, dres, dw, db, ws
+        args = [A] * 12
+        args[i] += off
+        assert lib.mz_group_norm_backward(None, ctypes.byref(norm), *args, 1 << 20) == -1, i
+    loss = L.Categorical(unroll=2, batch=3, target_positions=2, target_games=3, classes=5, dtype=1, index_bytes=8)
+    for i, off in enumerate((1, 2, 4, 4, 2, 2, 2, 1)):                 # logits, targets, game, position, weights, dloss, loss, dlogits
+        args = [A] * 8
+        args[i] += off
+        assert lib.mz_categorical_loss(None, ctypes.byref(loss), *args) == -1, i
+    table = (L.Tensor * 1)(L.Tensor(data=A, elements=4, dtype=0))
+    assert lib.mz_global_norm(None, 1, table, 0x1004, ws, A) == -1 and lib.mz_global_norm(None, 1, table, 0x1000, ws, A + 2) == -1

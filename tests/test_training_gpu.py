@@ -484,3 +484,23 @@ def test_a_set_is_not_made_inside_a_capture():
     with pytest.raises(MuZeroError, match='capture'):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             GradientSet([t])
+
+
+def test_a_set_whose_tensor_was_given_other_memory_is_refused():
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.training import GradientSet
+    a, b = torch.ones(8, device='cuda'), torch.ones(4, device='cuda')
+    kept = GradientSet([a, b])
+    kept.clip_by_global_norm(1.0)
+    b.set_(torch.zeros(4, device='cuda'))
+    for call in (kept.global_norm, lambda: kept.clip_by_global_norm(1.0)):
+        with pytest.raises(MuZeroError, match='other memory'):
+            call()
+
+
+def test_second_derivatives_of_the_loss_are_refused():
+    from muzero_amd.training import categorical_loss
+    z = torch.randn(4, 9, device='cuda', requires_grad=True)
+    (g,) = torch.autograd.grad(categorical_loss(z, block(4, 1, 9)[:, 0]).sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        g.sum().backward()
