@@ -542,7 +542,7 @@ int mz_group_norm_backward(void* stream, const mz_group_norm_t* config, const vo
  * [target_positions][target_games][classes] f32:
  *   loss[u][b] = w * sum over t_c != 0 of t_c * (log sum exp(z) - z_c),   dlogits = w * (sum(t) * softmax(z) - t).
  *   position, game: [batch] of index_bytes (4 or 8), each NULL = 0 and b.  A row outside the block gives NaN.
- *   weights [unroll][batch] f32 by weight_strides (NULL = 1); a row of weight 0 is not looked at: loss and gradient 0.
+ *   weights [unroll][batch] f32 by weight_strides (NULL = 1); a row of weight 0 has loss and gradient 0, whatever it holds.
  *   A row whose logits are all -inf (nothing left by a mask) has loss and gradient 0.
  *   dloss [unroll][batch] f32 by dloss_strides: factor of the gradient alone (NULL = 1).
  * out_loss [unroll][batch] f32 and out_dlogits (dense, `dtype`): either may be NULL.  classes in [1, 4096]. */

@@ -1,5 +1,5 @@
 """Layers of networks composed outside the built-in kernels, next to network.py's state-action encoders: group norm with
-an activation over channels-last states (csrc/mz_norm.hip), forward and backward."""
+an activation over channels-last states (csrc/mz_norm.hip), forward and backward.  Under capture, see training.py."""
 from typing import Optional
 
 import torch

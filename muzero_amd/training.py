@@ -1,6 +1,9 @@
 """Operators of a training step on the targets of replay.py: the categorical loss with its gradient (csrc/mz_loss.hip), the
 global gradient norm and clipping by it (csrc/mz_clip.hip).  The reference leaves them to Keras (training.py:13-51,157-204);
-the names follow its framework."""
+the names follow its framework.
+
+A forward pass that is being captured into a graph is refused where its backward pass would reach an autograd node of a stream
+outside the capture (an eager graph of the same leaves that is still alive)."""
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -25,7 +28,7 @@ def categorical_loss(logits: torch.Tensor, targets: torch.Tensor, game: Optional
     Without `game` and `position`, targets has the shape of logits.  With them, targets is a block [positions, games,
     classes] as replay.compute_targets returns it (policies, or values of a support), logits is [unroll, batch, classes], and
     row (u, b) meets targets[position[b] + u, game[b]]: no gathered copy.  An index outside the block gives NaN (the host
-    does not look at them).  weights broadcast over the rows; rows of weight 0 are not read and give 0 whatever they hold.  A
+    does not look at them).  weights broadcast over the rows; rows of weight 0 give 0 whatever they hold.  A
     class with target 0 adds nothing, also where its logit is -inf (an illegal move); a row whose logits are all -inf gives 0.
     A row of zero targets (past the end of a game) gives 0.  Differentiable once with respect to logits alone."""
     return _loss(_lib.native().categorical_loss, logits, targets, game, position, weights)
@@ -41,9 +44,9 @@ def categorical_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, game:
 
 
 # ---- global norm and clipping --------------------------------------------------------------------------------------------
-def _list(fn, *args):
+def _list(fn, tensors, *args):
     try:
-        return fn(*args)
+        return fn(list(tensors), *args)
     except TypeError:
         raise MuZeroError('tensors and out are lists of tensors (out may be None), max_norm is a number') from None
 
@@ -60,7 +63,7 @@ class GradientSet:
     used on several streams at once."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None) -> None:
-        self._set = _list(_lib.native().GradientSet, list(tensors), None if out is None else list(out))
+        self._set = _list(_lib.native().GradientSet, tensors, out)
 
     def global_norm(self) -> torch.Tensor:
         """sqrt of the sum of the squares of all elements of all tensors: a float32 scalar on the device."""
@@ -70,16 +73,19 @@ class GradientSet:
         """Writes every tensor times max_norm / global norm to its output where the norm is above max_norm, else unchanged,
         and returns the norm before clipping.  Where that is NaN every output is NaN; where it is infinite, finite elements
         become 0 and infinite ones NaN."""
-        return _list(self._set.clip_by_global_norm, max_norm)
+        try:
+            return self._set.clip_by_global_norm(max_norm)
+        except TypeError:
+            raise MuZeroError(f'max_norm must be a number, got {max_norm!r}') from None
 
 
 def global_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     """GradientSet(tensors).global_norm() for tensors that are others in every step: their table travels with the launch, 112
     tensors each, and nothing is uploaded."""
-    return _list(_lib.native().global_norm, list(tensors))
+    return _list(_lib.native().global_norm, tensors)
 
 
 def clip_by_global_norm(tensors: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """GradientSet(tensors, out).clip_by_global_norm(max_norm) in the same way: in place, or into `out`; returns the norm
     before clipping.  Tensors that are written may not share memory with others of the list."""
-    return _list(_lib.native().clip_by_global_norm, list(tensors), max_norm, None if out is None else list(out))
+    return _list(_lib.native().clip_by_global_norm, tensors, max_norm, out)

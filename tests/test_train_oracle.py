@@ -113,8 +113,8 @@ def test_gradient_set_refuses():
     from muzero_amd.exceptions import MuZeroError
     from muzero_amd.training import GradientSet, clip_by_global_norm, global_norm
     a, b = torch.zeros(3, 4), torch.zeros(5)
-    for tensors, out in (([], None), ([a.double()], None), ([a, 1.0], None), ([a[:, :2]], None), ([a, b], [a]), ([a], [b]),
-                         ([a], [a.half()]), ([torch.zeros(4).expand(3, 4)], None), ([a], [torch.zeros(4, 3).t()])):
+    for tensors, out in (([], None), (None, None), (a.numel(), None), ([a], 3), ([a], [1.0]), ([a.double()], None),
+                         ([a, 1.0], None), ([a[:, :2]], None), ([a, b], [a]), ([a], [b]), ([a], [a.half()]), ([torch.zeros(4).expand(3, 4)], None), ([a], [torch.zeros(4, 3).t()])):
         with pytest.raises(MuZeroError):
             GradientSet(tensors, out)
     with pytest.raises(MuZeroError):
