@@ -10,15 +10,15 @@ using mz_norm::Norm;
 using mz_norm::Plan;
 
 // The widest vectors of at most 16 bytes.  A group of V channels or more is cut into such vectors, its last one moved back to
-// end with it; smaller groups stand side by side in a vector where the channels are a multiple of it, else in one of two
-// channels or none.
+// end with it; smaller groups stand side by side in a vector where their size divides it, the last vector moved back to end
+// with the sample (10958 x 25 x 146 bf16 in groups of 2: backward 199 us in vectors of 2, 120 in vectors of 8).
 void choose_vector(const mz_group_norm_t* c, int* v, int* q) {
     const int most = 16 / mz::dtype_size(c->dtype), d = c->channels / c->groups;
     *q = 1;
     *v = most;
     if (d >= most) return;
-    if ((d & (d - 1)) == 0 && c->channels % most == 0) *q = most / d;
-    else if (d == 1 && c->channels % 2 == 0) *v = *q = 2;
+    if ((d & (d - 1)) == 0 && c->channels >= most) *q = most / d;
+    else if (d == 1 && c->channels > 1) *v = *q = 2;
     else
         while (*v > d) *v >>= 1;
 }
@@ -43,7 +43,7 @@ int log2_up(long v) {
 
 // Lanes of a workgroup of `threads`, and the vectors a thread then holds of a tile.
 int lay_out(Norm& d, int v, int item, int threads) {
-    const int dv = (d.U + v - 1) / v, lth = log2_up(threads), units = d.C / d.U;
+    const int dv = (d.U + v - 1) / v, lth = log2_up(threads), units = d.units;
     d.pieces = 1;
     d.samples = 1;
     d.ldv = log2_up(dv);
@@ -100,6 +100,7 @@ Plan plan(const mz_group_norm_t* c) {
     }
     choose_vector(c, &p.v, &p.q);
     d.U = p.q > 1 ? p.v : d.D;
+    d.units = (d.C + d.U - 1) / d.U;
     const int v = p.v, item = mz::dtype_size(c->dtype);
     // the smallest workgroup whose registers hold a tile, one wavefront without barriers if it may be
     for (const int threads : {64, 256, 512}) {
@@ -135,7 +136,7 @@ Plan plan(const mz_group_norm_t* c) {
 int64_t workspace_of(const Plan& p, bool backward) {
     const Norm& d = p.d;
     if (d.N == 0 || d.S == 0) return 0;
-    const int64_t parts = p.k ? 0 : d.N * d.G * d.splits * d.pieces * 2;
+    const int64_t parts = p.k ? 0 : d.N * d.units * p.q * d.splits * d.pieces * 2;
     if (!backward) return parts * (int64_t)sizeof(float);
     return ((p.k ? d.blocks : d.N * d.splits) * 2 * d.C + parts) * (int64_t)sizeof(float);
 }

@@ -11,8 +11,9 @@
 // many.  A thread keeps one vector of V channels and walks down the positions, so consecutive lanes read consecutive
 // addresses.  Vectors are as wide as an access can be (16 bytes) whatever D is: where D is no multiple of V, a group's last
 // vector is moved back to end with the group, and its first `dup` channels, which are the vector's before it too, count
-// nothing in the group's sums (they are stored twice, alike); where D is smaller than V, a vector holds Q = V / D groups with
-// a sum of its own each.  "Units" are what lanes share: a group, or the Q groups of a vector.  Vectors of a unit and units of
+// nothing in the group's sums (they are stored twice, alike); where D is a smaller power of two, a vector holds Q = V / D
+// groups with a sum of its own each, and a sample's last vector is moved back by whole groups (theirs is all stored twice,
+// alike).  "Units" are what lanes share: a group, or the Q groups of a vector.  Vectors of a unit and units of
 // a tile are padded to powers of two over the lanes: a lane's unit, vector and position come from bits of its number, and a
 // unit's sums are a butterfly over the other bits (group_sum), without index tables or divisions.  Two ways through:
 //   resident  the tile's values stay in registers between the statistics and the result: one launch, every input read once.
@@ -34,7 +35,7 @@ constexpr int kMostSplits = 64;
 
 struct Norm {
     long N, S;
-    int C, G, D, U, act, params_f32;          // U: channels of a unit
+    int C, G, D, U, units, act, params_f32;   // U: channels of a unit, the last of `units` ends with the sample
     float eps;
     long xs[2], rs[2], ds[2];
     // lanes: bits [vector in unit : ldv][unit in tile : lgs][position : lrows][sample : the rest]
@@ -56,11 +57,12 @@ struct Plan {
 struct Lane {
     int vec, unit, row, sample;               // vector of its unit, unit of its tile, first position, sample
     int g, ch, dup;                           // unit and first channel within the sample, channels that are another lane's too
+    int group;                                // first group of the unit
     int first, width;                         // this piece's first channel within its unit, and channels
     bool live;                                // not padding
 };
 
-template <int V>
+template <int V, int Q>
 __device__ Lane lane_of(const Norm& d, int tile) {
     Lane l;
     const int t = threadIdx.x;
@@ -77,13 +79,15 @@ __device__ Lane lane_of(const Norm& d, int tile) {
         l.width = d.U - l.first < V << d.ldv ? d.U - l.first : V << d.ldv;
     } else {
         l.g = tile * d.gs;
-        gs = d.C / d.U - l.g < gs ? d.C / d.U - l.g : gs;
+        gs = d.units - l.g < gs ? d.units - l.g : gs;
     }
     l.live = l.vec * V < l.width && l.unit < gs && l.sample < d.samples;
     if (l.unit < gs) l.g += l.unit;           // padding reads what a live lane reads, and counts nothing
     const int in_unit = l.first + (l.live ? l.vec * V : 0), from = in_unit < d.U - V ? in_unit : d.U - V;
     l.dup = in_unit - from;
-    l.ch = l.g * d.U + from;
+    const int begin = l.g * d.U;
+    l.ch = (begin < d.C - d.U ? begin : d.C - d.U) + from;
+    l.group = l.g * Q < d.G - Q ? l.g * Q : d.G - Q;
     return l;
 }
 
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
     const float inv = 1.f / ((float)d.S * (float)d.D);
     for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y)
         for (long n0 = (long)blockIdx.x * d.samples; n0 < d.N; n0 += (long)gridDim.x * d.samples) {
-            const Lane l = lane_of<V>(d, tile);
+            const Lane l = lane_of<V, Q>(d, tile);
             const int left = d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples;       // samples of this workgroup
             const bool live = l.live && l.sample < left;
             const int j = live ? l.sample : 0;
@@ -352,8 +356,8 @@ __global__ void __launch_bounds__(TH) norm_forward_kernel(Norm d) {
             for (int q = 0; q < Q; ++q) rs[q] = 1.f / sqrtf(sum[q] * inv + d.eps);
             if (!live) continue;
             if (d.mean && l.vec == 0 && l.row == 0) {
-                mz::store<float, Q>(d.mean + (n0 + j) * d.G + l.g * Q, mu);
-                mz::store<float, Q>(d.rstd + (n0 + j) * d.G + l.g * Q, rs);
+                mz::store<float, Q>(d.mean + (n0 + j) * d.G + l.group, mu);
+                mz::store<float, Q>(d.rstd + (n0 + j) * d.G + l.group, rs);
             }
             T* y = static_cast<T*>(d.y) + n0 * d.S * d.C;
             const int at = (j * S + l.row) * d.C + l.ch;
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(64) norm_forward_ahead_kernel(Norm d) {
     const int S = (int)d.S, step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
     for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y) {
-        const Lane l = lane_of<V>(d, tile);
+        const Lane l = lane_of<V, Q>(d, tile);
         const auto left = [&](long n0) { return d.N - n0 < d.samples ? (int)(d.N - n0) : d.samples; };      // samples of a set
         const auto load = [&](Held<T, V, K, 2>& h, long n0) {
             const int j = l.live && l.sample < left(n0) ? l.sample : 0;
@@ -414,8 +418,8 @@ __global__ void __launch_bounds__(64) norm_forward_ahead_kernel(Norm d) {
             for (int q = 0; q < Q; ++q) rs[q] = 1.f / sqrtf(sum[q] * inv + d.eps);
             if (live) {
                 if (d.mean && l.vec == 0 && l.row == 0) {
-                    mz::store<float, Q>(d.mean + (n0 + j) * d.G + l.g * Q, mu);
-                    mz::store<float, Q>(d.rstd + (n0 + j) * d.G + l.g * Q, rs);
+                    mz::store<float, Q>(d.mean + (n0 + j) * d.G + l.group, mu);
+                    mz::store<float, Q>(d.rstd + (n0 + j) * d.G + l.group, rs);
                 }
                 T* y = static_cast<T*>(d.y) + n0 * d.S * d.C;
                 const int at = (j * S + l.row) * d.C + l.ch;
@@ -441,7 +445,7 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
     const long block = blockIdx.x;
     int turn = 0;
     for (int tile = blockIdx.y; tile < d.tiles; tile += gridDim.y) {
-        const Lane l = lane_of<V>(d, tile);
+        const Lane l = lane_of<V, Q>(d, tile);
         float w[V], b[V], wq[V], s1[V] = {}, s2[V] = {};
         load_params<T, V>(d, l.ch, w, b);
 #pragma unroll
@@ -465,7 +469,7 @@ __global__ void __launch_bounds__(TH) norm_backward_kernel(Norm d) {
             const int j = live ? l.sample : 0;
             auto &xv = held.v[0], &gv = held.v[1], &rv = held.v[2];
             float mu[Q], rs[Q], aq[2 * Q] = {};
-            load_stats(d, (n0 + j) * d.G + l.g * Q, mu, rs);
+            load_stats(d, (n0 + j) * d.G + l.group, mu, rs);
             with_activation(d.act, [&](auto act) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
@@ -522,7 +526,7 @@ __device__ inline void for_each_part(const Norm& d, F f) {
 }
 // where (split, piece) of a unit stands among its splits * pieces partial results
 __device__ inline long part_at(const Norm& d, const Part& p, const Lane& l) {
-    return ((p.n * (d.C / d.U) + l.g) * d.splits + p.split) * d.pieces + (d.pieces > 1 ? p.tile % d.pieces : 0);
+    return ((p.n * d.units + l.g) * d.splits + p.split) * d.pieces + (d.pieces > 1 ? p.tile % d.pieces : 0);
 }
 
 constexpr int kBatch = 4;                       // vectors of a thread under way at once
@@ -540,7 +544,7 @@ __global__ void __launch_bounds__(kSplitThreads) norm_stats_kernel(Norm d) {
     __shared__ float scratch[2][kSplitThreads * Q];
     const int step = 1 << d.lrows;
     for_each_part(d, [&](const Part& p) {
-        const Lane l = lane_of<V>(d, p.tile);
+        const Lane l = lane_of<V, Q>(d, p.tile);
         float count = 0.f, mean[Q] = {}, m2[Q] = {};
         if (l.live) {
             const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
@@ -593,12 +597,12 @@ __global__ void __launch_bounds__(kSplitThreads) norm_apply_kernel(Norm d) {
     const int step = 1 << d.lrows;
     const float inv = 1.f / ((float)d.S * (float)d.D);
     for_each_part(d, [&](const Part& p) {
-        const Lane l = lane_of<V>(d, p.tile);
+        const Lane l = lane_of<V, Q>(d, p.tile);
         const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
         const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
         // the unit's parts, over its lanes (a part's share of the values: its positions times its channels)
         const int parts = d.splits * d.pieces, lanes = 1 << (d.ldv + d.lrows), mine = (l.row << d.ldv) + l.vec;
-        const float* ws = d.ws + 2 * Q * (p.n * (d.C / d.U) + l.g) * parts;
+        const float* ws = d.ws + 2 * Q * (p.n * d.units + l.g) * parts;
         const auto count = [&](int e) {
             const int split = d.pieces > 1 ? e / d.pieces : e, from = ((e - split * d.pieces) << d.ldv) * V;
             const long positions = split * d.chunk + d.chunk < d.S ? d.chunk : d.S - split * d.chunk;
@@ -626,8 +630,8 @@ __global__ void __launch_bounds__(kSplitThreads) norm_apply_kernel(Norm d) {
         for (int q = 0; q < Q; ++q) rs[q] = 1.f / sqrtf(a[q] * inv + d.eps);
         if (!l.live) return;
         if (d.mean && p.split == 0 && l.vec == 0 && l.row == 0 && (d.pieces == 1 || p.tile % d.pieces == 0)) {
-            mz::store<float, Q>(d.mean + p.n * d.G + l.g * Q, mu);
-            mz::store<float, Q>(d.rstd + p.n * d.G + l.g * Q, rs);
+            mz::store<float, Q>(d.mean + p.n * d.G + l.group, mu);
+            mz::store<float, Q>(d.rstd + p.n * d.G + l.group, rs);
         }
         float w[V], b[V];
         load_params<T, V>(d, l.ch, w, b);
@@ -652,14 +656,14 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_sums_kernel(Norm d) {
     __shared__ float scratch[2][kSplitThreads * (V > 2 * Q ? V : 2 * Q)];
     const int step = 1 << d.lrows;
     for_each_part(d, [&](const Part& p) {
-        const Lane l = lane_of<V>(d, p.tile);
+        const Lane l = lane_of<V, Q>(d, p.tile);
         float s1[V] = {}, s2[V] = {}, w[V], b[V], wq[V], aq[2 * Q] = {};
         load_params<T, V>(d, l.ch, w, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) wq[i] = Q == 1 && i < l.dup ? 0.f : w[i];
         if (l.live) {
             float mu[Q], rs[Q];
-            load_stats(d, p.n * d.G + l.g * Q, mu, rs);
+            load_stats(d, p.n * d.G + l.group, mu, rs);
             const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
             const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
             const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
@@ -708,12 +712,12 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
     const float inv = 1.f / ((float)d.S * (float)d.D);
     int turn = 0;
     for_each_part(d, [&](const Part& p) {
-        const Lane l = lane_of<V>(d, p.tile);
+        const Lane l = lane_of<V, Q>(d, p.tile);
         const T* x = static_cast<const T*>(d.x) + p.n * d.xs[0] + l.ch;
         const T* res = d.res ? static_cast<const T*>(d.res) + p.n * d.rs[0] + l.ch : nullptr;
         const T* dy = static_cast<const T*>(d.dy) + p.n * d.ds[0] + l.ch;
         const int parts = d.splits * d.pieces;
-        const float* ws = d.ws + d.N * d.splits * 2 * d.C + 2 * Q * (p.n * (d.C / d.U) + l.g) * parts;
+        const float* ws = d.ws + d.N * d.splits * 2 * d.C + 2 * Q * (p.n * d.units + l.g) * parts;
         float aq[2 * Q] = {}, mu[Q], rs[Q];
         if (l.unit < d.gs)
             for (int e = (l.row << d.ldv) + l.vec; e < parts; e += 1 << (d.ldv + d.lrows)) {
@@ -726,7 +730,7 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
         if (!l.live) return;
 #pragma unroll
         for (int q = 0; q < 2 * Q; ++q) aq[q] *= inv;
-        load_stats(d, p.n * d.G + l.g * Q, mu, rs);
+        load_stats(d, p.n * d.G + l.group, mu, rs);
         float w[V], b[V];
         load_params<T, V>(d, l.ch, w, b);
         const long out = p.n * d.S * d.C + l.ch;

@@ -42,6 +42,13 @@ CASES += [
     (2, (400,), 130, 1, BF16, 'relu', True, 'f32'), (2, (90,), 7, 1, F16, 'gelu', True, None), (3, (129,), 1026, 2, F32, 'relu', False, 'f32'),
 ]
 
+# several groups in a vector, the last vector moved back to end with the sample
+CASES += [
+    (5, (9,), 37, 37, BF16, 'gelu', True, 'same'), (3, (4,), 21, 21, F32, 'silu', False, 'f32'), (3, (5,), 1002, 501, F32, 'relu', True, 'f32'),
+    (700, (2,), 10, 5, F16, 'tanh', True, 'f32'), (2, (1400,), 9, 9, F32, 'gelu', True, 'f32'), (1, (2500,), 35, 35, BF16, 'relu', False, 'f32'),
+    (2, (2000,), 22, 11, F16, 'silu', True, 'same'), (1, (1100,), 1028, 257, BF16, None, True, 'f32'), (3, (100,), 5, 5, F16, 'relu', True, 'f32'),
+]
+
 
 def make(case, seed=0):
     N, shape, C, G, dtype, activation, residual, params = case
