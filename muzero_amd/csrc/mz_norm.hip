@@ -55,23 +55,28 @@ int lay_out(Norm& d, int v, int item, int threads) {
         d.tiles = units * d.pieces;
         return 0;
     }
-    // Units of a tile: those of a 128-byte line, or more where that leaves fewer lanes idle over the positions, the padding of
-    // the tiles and the samples side by side -- unless there are too few tiles to begin with, or a thread would then hold more
-    // vectors than the kernels that read ahead do (nine positions on eight rows of lanes: two vectors a thread, nine sixteenths
-    // of them live; on four rows three, three quarters: backward of 34722 x 9 x 128 f32 in groups of 4 148 -> 116 us).
+    // Units of a tile and positions side by side: the units of a 128-byte line, or more, and as many positions as there are
+    // lanes, or fewer beside more samples, whatever leaves fewest lanes idle over the positions, the padding of the tiles and
+    // the samples -- unless there are too few workgroups to begin with, or a thread would then hold more vectors than the
+    // kernels that read ahead do (nine positions on eight rows of lanes: two vectors a thread, nine sixteenths of them live; on
+    // four rows three, three quarters).  The half a step is what sums over the lanes cost: they are shared by more vectors.
+    // Backward: 34722 x 9 x 128 f32 in groups of 4 148 -> 116 us; 277777 x 9 x 16 bf16 137 -> 87; 104166 x 3 x 128 f32 179 -> 110.
     const int all = log2_up(units), room = lth - d.ldv, most = all < room ? all : room;
     const int line = log2_up((128 + (long)d.U * item - 1) / ((long)d.U * item)), least = line < most ? line : most, ls = log2_up(d.S);
     double best = INFINITY;
     long k = 0;
     for (int lgs = least; lgs <= most; ++lgs) {
-        const int tiles = (units + (1 << lgs) - 1) >> lgs, lrows = lth - d.ldv - lgs < ls ? lth - d.ldv - lgs : ls;
-        const long steps = (d.S + (1L << lrows) - 1) >> lrows;
-        const double cost = (double)tiles * (double)steps / (double)(1 << (lth - d.ldv - lgs - lrows));
-        if (lgs > least && (cost >= best || steps > 4 || d.N * tiles < 2048)) continue;
-        best = cost;
-        k = steps;
-        d.lgs = lgs;
-        d.lrows = lrows;
+        const int tiles = (units + (1 << lgs) - 1) >> lgs, widest = room - lgs < ls ? room - lgs : ls;
+        for (int lrows = widest; lrows >= 0; --lrows) {
+            const long steps = (d.S + (1L << lrows) - 1) >> lrows, samples = 1L << (room - lgs - lrows);
+            const double cost = (double)tiles * ((double)steps + 0.5) / (double)samples;
+            const bool first = lgs == least && lrows == widest;
+            if (!first && (cost >= best || steps > 4 || d.N * tiles < 2048 * (lrows < widest ? samples : 1))) continue;
+            best = cost;
+            k = steps;
+            d.lgs = lgs;
+            d.lrows = lrows;
+        }
     }
     d.samples = 1 << (lth - d.ldv - d.lgs - d.lrows);
     d.tiles = (units + (1 << d.lgs) - 1) >> d.lgs;

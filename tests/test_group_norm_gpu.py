@@ -49,6 +49,12 @@ CASES += [
     (2, (2000,), 22, 11, F16, 'silu', True, 'same'), (1, (1100,), 1028, 257, BF16, None, True, 'f32'), (3, (100,), 5, 5, F16, 'relu', True, 'f32'),
 ]
 
+# enough samples for fewer positions side by side: several vectors a thread, samples that do not fill the last set
+CASES += [
+    (2500, (9,), 16, 4, BF16, 'relu', True, 'f32'), (4099, (3,), 128, 16, F32, 'silu', True, 'f32'), (9001, (3, 3), 3, 3, F16, 'gelu', False, 'same'),
+    (2053, (5,), 64, 16, F16, 'tanh', True, 'f32'), (6007, (7,), 40, 8, BF16, 'relu', True, 'f32'), (8195, (10,), 20, 5, F32, None, False, None),
+]
+
 
 def make(case, seed=0):
     N, shape, C, G, dtype, activation, residual, params = case
