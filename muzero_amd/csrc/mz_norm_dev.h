@@ -15,7 +15,8 @@
 // groups with a sum of its own each, and a sample's last vector is moved back by whole groups (theirs is all stored twice,
 // alike).  "Units" are what lanes share: a group, or the Q groups of a vector.  Vectors of a unit and units of
 // a tile are padded to powers of two over the lanes: a lane's unit, vector and position come from bits of its number, and a
-// unit's sums are a butterfly over the other bits (group_sum), without index tables or divisions.  Two ways through:
+// unit's sums are a butterfly over the bits of its vectors and positions (group_sum), without index tables or divisions.  Two
+// ways through:
 //   resident  the tile's values stay in registers between the statistics and the result: one launch, every input read once.
 //   split     samples too large for that (K vectors a thread do not hold the tile): positions are cut into chunks over
 //             several workgroups; a first launch leaves each chunk's partial sums, a second adds them up and reads again.
@@ -107,16 +108,17 @@ __device__ inline void group_sum(float (&v)[N], const Norm& d, float* scratch) {
 #pragma unroll
         for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m);
     if (TH == 64) return;
-    const int t = threadIdx.x, groups = (pitch - 1) & ~(dvp - 1) & ~63;       // bits of the wavefront's number that are a unit's
-    // one slot for each unit of a wavefront
-    const int slot = (t & 63 & (pitch - 1)) >> (d.ldv < 6 ? d.ldv : 6);
+    // a unit's lanes differ in vector and position alone: wavefronts whose numbers differ in a unit's or a sample's bit stay apart
+    const int t = threadIdx.x, sample = d.ldv + d.lgs + d.lrows, apart = ~((dvp - 1) | ((1 << d.lrows) - 1) * pitch) & ~63;
+    // one slot for each unit and sample of a wavefront
+    const int slot = ((t & 63 & (pitch - 1)) >> (d.ldv < 6 ? d.ldv : 6)) + (((t & 63) >> sample) << d.lgs);
 #pragma unroll
     for (int k = 0; k < N; ++k) scratch[(t >> 6) * 64 * N + slot * N + k] = v[k];      // lanes of one slot hold the same value
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = 0.f;
     for (int w = 0; w < TH / 64; ++w)
-        if ((((w << 6) ^ t) & groups) == 0)
+        if ((((w << 6) ^ t) & apart) == 0)
 #pragma unroll
             for (int k = 0; k < N; ++k) v[k] += scratch[w * 64 * N + slot * N + k];
 }
