@@ -527,6 +527,10 @@ typedef struct mz_group_norm {
 } mz_group_norm_t;
 /* Bytes of workspace that the forward / backward call takes (0: none), or a negative mz_status. */
 int64_t mz_group_norm_workspace(const mz_group_norm_t* config, int32_t backward);
+/* Inspection (tests): how a workgroup's lanes share a state under `config`.  out8_host (HOST): [0] threads, [1] vectors that a
+ * thread holds (0: positions split over workgroups), lanes side by side along [2] samples, [3] positions, [4] groups (or
+ * vectors of several) and [5] vectors of a group, [6] pieces of a group wider than a workgroup, [7] chunks of positions. */
+int mz_debug_group_norm_layout(const mz_group_norm_t* config, int32_t* out8_host);
 /* out_mean, out_rstd: [batch][groups] f32 for the backward call, both or neither NULL. */
 int mz_group_norm_forward(void* stream, const mz_group_norm_t* config, const void* x, const void* residual,
                           const void* weight, const void* bias, void* out_y, float* out_mean, float* out_rstd,

@@ -158,6 +158,7 @@ PROTOTYPES = {
     'mz_replay_targets': (ctypes.c_int, [c_void_p, ctypes.POINTER(ReplayConfig)] + [c_void_p] * 12),
     # the configurations of the training operators: a structure by reference, or its bytes
     'mz_group_norm_workspace': (c_int64, [c_void_p, c_int32]),
+    'mz_debug_group_norm_layout': (ctypes.c_int, [c_void_p, c_void_p]),
     'mz_group_norm_forward': (ctypes.c_int, [c_void_p, c_void_p] + [c_void_p] * 8 + [c_int64]),
     'mz_group_norm_backward': (ctypes.c_int, [c_void_p, c_void_p] + [c_void_p] * 12 + [c_int64]),
     'mz_categorical_loss': (ctypes.c_int, [c_void_p, c_void_p] + [c_void_p] * 8),

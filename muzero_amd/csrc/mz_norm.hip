@@ -41,8 +41,9 @@ int log2_up(long v) {
     return l;
 }
 
-// Lanes of a workgroup of `threads`, and the vectors a thread then holds of a tile.
-int lay_out(Norm& d, int v, int item, int threads) {
+// Lanes of a workgroup of `threads`, and the vectors a thread then holds of a tile.  The split kernels take one sample a
+// workgroup: with `several` false all lanes that units leave are positions, the ones past the last idle.
+int lay_out(Norm& d, int v, int item, int threads, bool several) {
     const int dv = (d.U + v - 1) / v, lth = log2_up(threads), units = d.units;
     d.pieces = 1;
     d.samples = 1;
@@ -66,8 +67,8 @@ int lay_out(Norm& d, int v, int item, int threads) {
     double best = INFINITY;
     long k = 0;
     for (int lgs = least; lgs <= most; ++lgs) {
-        const int tiles = (units + (1 << lgs) - 1) >> lgs, widest = room - lgs < ls ? room - lgs : ls;
-        for (int lrows = widest; lrows >= 0; --lrows) {
+        const int tiles = (units + (1 << lgs) - 1) >> lgs, widest = room - lgs < ls || !several ? room - lgs : ls;
+        for (int lrows = widest; lrows >= (several ? 0 : widest); --lrows) {
             const long steps = (d.S + (1L << lrows) - 1) >> lrows, samples = 1L << (room - lgs - lrows);
             const double cost = (double)tiles * ((double)steps + 0.5) / (double)samples;
             const bool first = lgs == least && lrows == widest;
@@ -109,10 +110,11 @@ Plan plan(const mz_group_norm_t* c) {
     const int v = p.v, item = mz::dtype_size(c->dtype);
     // the smallest workgroup whose registers hold a tile, one wavefront without barriers if it may be
     for (const int threads : {64, 256, 512}) {
-        const int k = lay_out(d, v, item, threads);
+        const int k = lay_out(d, v, item, threads, true);
         const int64_t reach = (int64_t(1) << 31) / item - d.C;                 // elements that a 32-bit byte offset spans
         bool near = true;
-        for (const long* s : {d.xs, d.rs, d.ds}) near &= spans(s[0], d.samples - 1, reach / 2) && spans(s[1], d.S - 1, reach / 2);
+        const long last = (d.samples < d.N ? d.samples : d.N) - 1;             // of a workgroup's samples
+        for (const long* s : {d.xs, d.rs, d.ds}) near &= spans(s[0], last, reach / 2) && spans(s[1], d.S - 1, reach / 2);
         near &= spans(d.S * d.C, d.samples, reach);
         if (k < 1 || k > 8 || !near) continue;
         p.threads = threads;
@@ -125,7 +127,7 @@ Plan plan(const mz_group_norm_t* c) {
         d.splits = 1;
         return p;
     }
-    lay_out(d, v, item, kSplitThreads);
+    lay_out(d, v, item, kSplitThreads, false);
     p.threads = kSplitThreads;
     p.k = 0;
     const long tiles = d.N * d.tiles > 0 ? d.N * d.tiles : 1, most = (d.S + (8L << d.lrows) - 1) / (8L << d.lrows);
@@ -165,6 +167,17 @@ extern "C" {
 int64_t mz_group_norm_workspace(const mz_group_norm_t* c, int32_t backward) {
     const int bad = check(c);
     return bad ? bad : workspace_of(plan(c), backward != 0);
+}
+
+int mz_debug_group_norm_layout(const mz_group_norm_t* c, int32_t* out8_host) {
+    const int bad = check(c);
+    if (bad) return bad;
+    MZ_REQUIRE(out8_host, "out8_host is NULL");
+    const Plan p = plan(c);
+    const Norm& d = p.d;
+    const int32_t out[8] = {p.threads, p.k, d.samples, 1 << d.lrows, 1 << d.lgs, 1 << d.ldv, d.pieces, d.splits};
+    for (int i = 0; i < 8; ++i) out8_host[i] = out[i];
+    return MZ_OK;
 }
 
 int mz_group_norm_forward(void* stream, const mz_group_norm_t* c, const void* x, const void* residual, const void* weight,

@@ -64,3 +64,36 @@ def test_a_sample_does_not_see_the_others(case):
             check('y', got[0], o.y, o.off_y, x.dtype)
             check('dx', got[1], want['dx'], off['dx'], x.dtype)
             check('dresidual', got[2], want['dresidual'], off['dresidual'], x.dtype)
+
+
+def spread(t, batch_stride, position_stride=None):
+    """t [N, S, C], its samples (and positions) that many elements apart."""
+    N, S, C = t.shape
+    position_stride = position_stride or C
+    memory = torch.empty((N - 1) * batch_stride + (S - 1) * position_stride + C, dtype=t.dtype, device='cuda')
+    return memory.as_strided(t.shape, (batch_stride, position_stride, 1)).copy_(t)
+
+
+# small samples that lie farther apart than 32-bit offsets reach from the first of a workgroup to its last: a step of each game
+# out of a large buffer, or positions on the far side of one
+FAR = [
+    ((3, (4,), 16, 4, F32, 'silu', True, 'f32'), 200_000_000, None), ((20, (1,), 16, 4, F32, 'tanh', True, 'f32'), 20_000_000, None),
+    ((3, (9,), 16, 4, BF16, 'gelu', True, 'f32'), 600_000_000, None), ((7, (1,), 24, 24, F16, 'silu', True, 'same'), 100_000_001, None),
+    ((2, (1,), 300, 1, F32, None, True, 'f32'), 300_000_000, None), ((3, (5,), 20, 10, BF16, 'silu', True, 'f32'), 600_000_000, None),
+    ((70, (2,), 8, 2, F32, 'silu', True, 'f32'), 40_000_001, None),
+    ((3, (3,), 64, 16, F16, 'gelu', True, 'f32'), 64, 400_000_000), ((2, (2,), 37, 37, BF16, 'tanh', True, 'same'), 37, 700_000_001),
+]
+
+
+@pytest.mark.parametrize('which', ['x', 'residual', 'dy', 'all'])
+@pytest.mark.parametrize('case', FAR, ids=lambda c: name_of(c[0]) + f'-{c[1]}-{c[2]}')
+def test_samples_and_positions_far_apart(case, which):
+    shape, batch_stride, position_stride = case
+    x, G, w, b, activation, res, dy = make(shape, 23)
+    if which in ('x', 'all'):
+        x = spread(x, batch_stride, position_stride)
+    if which in ('residual', 'all'):
+        res = spread(res, batch_stride, position_stride)
+    if which in ('dy', 'all'):
+        dy = spread(dy, batch_stride, position_stride)
+    run_and_check(x, G, w, b, activation, res, dy)
