@@ -58,6 +58,22 @@ void require_hip(const c10::Device& d) {
     if (!d.is_cuda()) refuse("the tensors must be on a HIP device, not ", d, "; muzero_amd has no CPU fallback");
 }
 
+// What the kernels cannot take from t's memory, or nullptr.  Derivatives that travel with a tensor instead of a graph would be
+// lost without a word.
+const char* unreadable(const Tensor& t) {
+    if (t.layout() != at::kStrided) return "is not a strided tensor";
+    if (!t.has_storage()) return "has no memory of its own (a tensor inside a transform of torch.func, for instance)";
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+        return "carries a forward-mode derivative: muzero_amd's training operators are differentiable in reverse mode alone";
+    return nullptr;
+}
+void require_readable(const char* name, const Tensor& t) {
+    if (const char* why = unreadable(t)) refuse(name, " ", why);
+}
+void require_readable(const char* name, const OptTensor& t) {
+    if (t) require_readable(name, *t);
+}
+
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* data(const OptTensor& t) { return t ? data(*t) : nullptr; }
 bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
@@ -182,6 +198,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &residual = saved[3], &stats = saved[4];
         mz_group_norm_t config;
         memcpy(&config, ctx->saved_data["config"].toStringRef().data(), sizeof(config));
+        require_readable("the gradient", dys[0]);
         const Tensor dy = states(dys[0], config.dy_strides);
         const auto like = [&](int input, const Tensor& t) {
             return ctx->needs_input_grad(input) ? at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)) : Tensor();
@@ -215,6 +232,10 @@ int activation_of(const std::optional<std::string>& name) {
 
 Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
                   const std::optional<std::string>& activation, const OptTensor& residual) {
+    require_readable("x", x);
+    require_readable("weight", weight);
+    require_readable("bias", bias);
+    require_readable("residual", residual);
     require_type("x", x, dtype_of(x) >= 0, "float32, float16 or bfloat16");
     if (x.dim() < 2) refuse("x must be [B, ..., C], got shape ", x.sizes());
     const int64_t channels = x.size(-1);
@@ -279,6 +300,11 @@ Tensor rows_of(const Tensor& t, int64_t (&strides)[2]) {
 }
 
 LossCall describe(const Tensor& logits, const Tensor& targets, const OptTensor& game, const OptTensor& position, const OptTensor& weights) {
+    require_readable("logits", logits);
+    require_readable("targets", targets);
+    require_readable("game", game);
+    require_readable("position", position);
+    require_readable("weights", weights);
     require_type("logits", logits, dtype_of(logits) >= 0, "float32, float16 or bfloat16");
     const c10::Device device = logits.device();
     const auto shape = logits.sizes();
@@ -375,6 +401,7 @@ struct CategoricalLoss : torch::autograd::Function<CategoricalLoss> {
         c.game = saved[2];
         c.position = saved[3];
         c.weights = saved[4];
+        require_readable("the gradient", dloss[0]);
         const Tensor grad = loss_run(c, false, true, dloss[0]).second;
         return once({grad, Tensor()}, {c.logits, dloss[0]});
     }
@@ -423,6 +450,7 @@ struct TensorList {
         described.reserve(n);
         for (size_t i = 0; i < n; ++i) {
             const Tensor& t = tensors[i];
+            if (const char* why = unreadable(t)) refuse("tensor ", i, " ", why);
             if (dtype_of(t) < 0) refuse("tensor ", i, ": expected float32, float16 or bfloat16, got ", t.scalar_type());
             if (t.device() != device) refuse("tensor ", i, " is on ", t.device(), ", expected ", device);
             if (!dense(t)) refuse("tensor ", i, " is not dense: shape ", t.sizes(), ", strides ", t.strides());
@@ -433,6 +461,7 @@ struct TensorList {
             if (out.size() != n) refuse(n, " tensors, ", out.size(), " outputs");
             for (size_t i = 0; i < n; ++i) {
                 const Tensor &t = tensors[i], &u = out[i];
+                if (const char* why = unreadable(u)) refuse("output ", i, " ", why);
                 if (u.scalar_type() != t.scalar_type() || u.device() != device || u.sizes() != t.sizes() ||
                     !((u.is_contiguous() && t.is_contiguous()) || u.strides() == t.strides()))
                     refuse("output ", i, " must be like its tensor: ", t.scalar_type(), " ", t.sizes(), ", strides ", t.strides(), ", on ", device);

@@ -1,0 +1,53 @@
+"""Calls of the training operators that would return results without what belongs to them (a derivative, a recorded operation, a
+sign) or read other memory than they were given: refused, before anything is launched and whatever the device."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from muzero_amd.exceptions import MuZeroError
+
+
+def calls(wrap=lambda t: t):
+    """name -> a call of each operator, one of its tensors wrapped."""
+    from muzero_amd.layers import group_norm
+    from muzero_amd.training import GradientSet, categorical_loss, categorical_loss_and_grad, clip_by_global_norm, global_norm
+    x, w, z, t = torch.zeros(2, 3, 8), torch.ones(8), torch.zeros(4, 5), torch.ones(4, 5)
+    return {'x': lambda: group_norm(wrap(x), 2), 'weight': lambda: group_norm(x, 2, wrap(w)), 'bias': lambda: group_norm(x, 2, w, wrap(w)),
+            'residual': lambda: group_norm(x, 2, residual=wrap(x)), 'logits': lambda: categorical_loss(wrap(z), t),
+            'targets': lambda: categorical_loss(z, wrap(t)), 'weights': lambda: categorical_loss(z, t, weights=wrap(torch.ones(4))),
+            'both': lambda: categorical_loss_and_grad(wrap(z), t), 'norm': lambda: global_norm([x, wrap(w)]),
+            'clip': lambda: clip_by_global_norm([wrap(x), w], 1.0), 'out': lambda: clip_by_global_norm([x], 1.0, [wrap(x.clone())]),
+            'set': lambda: GradientSet([x, wrap(w)])}
+
+
+@pytest.mark.parametrize('name', calls())
+def test_forward_mode_derivatives(name):
+    with forward_ad.dual_level():
+        with pytest.raises(MuZeroError, match='forward-mode'):
+            calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))[name]()
+
+
+@pytest.mark.parametrize('name', calls())
+def test_tensors_without_memory_of_their_own(name):
+    for transform in (lambda f: torch.func.vmap(f)(torch.zeros(3)), lambda f: torch.func.grad(f)(torch.tensor(0.0)),
+                      lambda f: torch.func.jvp(f, (torch.tensor(0.0),), (torch.tensor(1.0),))):
+        with pytest.raises(MuZeroError, match='torch.func'):
+            transform(lambda s: calls(lambda t: t + s)[name]())
+    with pytest.raises(MuZeroError, match='strided'):
+        calls(lambda t: t.to_sparse())[name]()
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_on_the_device():
+    from muzero_amd.layers import group_norm
+    from muzero_amd.training import categorical_loss
+    x, z = torch.randn(2, 3, 8, device='cuda', requires_grad=True), torch.randn(4, 5, device='cuda', requires_grad=True)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t.detach(), torch.ones_like(t))
+        for call in (lambda: group_norm(dual(x), 2), lambda: categorical_loss(dual(z), torch.ones_like(z))):
+            with pytest.raises(MuZeroError, match='forward-mode'):
+                call()
+        for y, leaf in ((group_norm(x, 2), x), (categorical_loss(z, torch.ones(4, 5, device='cuda')), z)):
+            with pytest.raises(RuntimeError, match='forward-mode'):        # a tangent of the gradient
+                torch.autograd.grad(y, leaf, dual(y))
+        assert torch.isfinite(group_norm(forward_ad.unpack_dual(dual(x)).primal, 2)).all()
