@@ -4,6 +4,8 @@
 // it, and moves Python's objects between the cores of both (120 to 130 us a forward and backward pass of a small state,
 // of which an empty node takes 22 to 46).
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -72,6 +74,17 @@ void require_readable(const char* name, const Tensor& t) {
 }
 void require_readable(const char* name, const OptTensor& t) {
     if (t) require_readable(name, *t);
+}
+
+// A recording of torch's operations would hold the outputs' allocation and not the kernel that fills them.
+void refuse_while_recording() {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    if (torch::jit::tracer::isTracing()) refuse("muzero_amd's operators cannot be recorded by torch.jit.trace");
+    if (TorchDispatchModeTLS::any_modes_set() &&
+        (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) ||
+         TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL)))
+        refuse("muzero_amd's operators cannot be recorded by torch.fx or torch.export, nor run on fake tensors");
 }
 
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -232,6 +245,7 @@ int activation_of(const std::optional<std::string>& name) {
 
 Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
                   const std::optional<std::string>& activation, const OptTensor& residual) {
+    refuse_while_recording();
     require_readable("x", x);
     require_readable("weight", weight);
     require_readable("bias", bias);
@@ -300,6 +314,7 @@ Tensor rows_of(const Tensor& t, int64_t (&strides)[2]) {
 }
 
 LossCall describe(const Tensor& logits, const Tensor& targets, const OptTensor& game, const OptTensor& position, const OptTensor& weights) {
+    refuse_while_recording();
     require_readable("logits", logits);
     require_readable("targets", targets);
     require_readable("game", game);
@@ -444,6 +459,7 @@ struct TensorList {
     c10::Device device = at::kCPU;
 
     TensorList(std::vector<Tensor> t, std::optional<std::vector<Tensor>> o) : tensors(std::move(t)) {
+        refuse_while_recording();
         const size_t n = tensors.size();
         if (n < 1 || n > MZ_GLOBAL_NORM_MAX_TENSORS) refuse("1 to ", MZ_GLOBAL_NORM_MAX_TENSORS, " tensors, got ", n);
         device = tensors[0].device();
@@ -489,6 +505,7 @@ struct TensorList {
     // call(stream, workspace, its size, norm) -> status
     template <typename F>
     Tensor run(F call) const {
+        refuse_while_recording();
         const auto options = at::TensorOptions().device(device);
         const Tensor ws = at::empty({MZ_GLOBAL_NORM_WORKSPACE}, options.dtype(at::kByte)), norm = at::empty({}, options.dtype(at::kFloat));
         const On on(device);

@@ -51,3 +51,40 @@ def test_forward_mode_derivatives_on_the_device():
             with pytest.raises(RuntimeError, match='forward-mode'):        # a tangent of the gradient
                 torch.autograd.grad(y, leaf, dual(y))
         assert torch.isfinite(group_norm(forward_ad.unpack_dual(dual(x)).primal, 2)).all()
+
+
+def recordings(call):
+    """The call under everything that records torch's operations."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    s = torch.zeros(())
+    yield lambda: torch.jit.trace(call, (s,), check_trace=False)
+    yield lambda: make_fx(call)(s)
+    yield lambda: make_fx(call, tracing_mode='fake')(s)
+
+    def fake():
+        with FakeTensorMode(allow_non_fake_inputs=True):
+            call(s)
+    yield fake
+
+
+@pytest.mark.parametrize('name', calls())
+def test_recorded_calls(name):
+    for record in recordings(lambda s: calls()[name]()):
+        with pytest.raises(MuZeroError, match='cannot be recorded'):
+            record()
+
+
+@pytest.mark.gpu
+def test_recorded_calls_on_the_device():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from muzero_amd.layers import group_norm
+    from muzero_amd.training import GradientSet, categorical_loss, clip_by_global_norm
+    x, z = torch.randn(2, 3, 8, device='cuda'), torch.randn(4, 5, device='cuda')
+    t, kept = torch.ones_like(z), GradientSet([x.clone()])
+    for call in (lambda x, z: group_norm(x, 2), lambda x, z: categorical_loss(z, t), lambda x, z: clip_by_global_norm([x], 1.0),
+                 lambda x, z: kept.global_norm(), lambda x, z: kept.clip_by_global_norm(1.0)):
+        for record in (lambda: torch.jit.trace(call, (x, z), check_trace=False), lambda: make_fx(call)(x, z)):
+            with pytest.raises(MuZeroError, match='cannot be recorded'):
+                record()
+        assert torch.isfinite(call(x.clone(), z)).all()                    # and not refused any longer
