@@ -516,6 +516,7 @@ typedef enum mz_activation { MZ_ACT_NONE = 0, MZ_ACT_RELU = 1, MZ_ACT_SILU = 2, 
  * x, residual and dy (its gradient) are [batch][positions][channels] of `dtype` with a stride (in elements) for batch
  * and position each and adjacent channels; strides of 0 repeat.  y, dx, dresidual are dense and may not overlap inputs.
  * weight, bias: [channels] of `param_dtype` (MZ_F32 or `dtype`), each NULL = 1 and 0; residual NULL = none. */
+#define MZ_GROUP_NORM_MAX_CHANNELS 16777216
 typedef struct mz_group_norm {
     int64_t batch, positions;
     int32_t channels, groups;

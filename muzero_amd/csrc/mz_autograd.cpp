@@ -253,6 +253,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, cons
     require_type("x", x, dtype_of(x) >= 0, "float32, float16 or bfloat16");
     if (x.dim() < 2) refuse("x must be [B, ..., C], got shape ", x.sizes());
     const int64_t channels = x.size(-1);
+    if (channels > MZ_GROUP_NORM_MAX_CHANNELS) refuse("at most ", MZ_GROUP_NORM_MAX_CHANNELS, " channels, got ", channels);
     if (groups < 1 || channels < 1 || channels % groups) refuse(channels, " channels cannot be split into ", groups, " groups");
     const int act = activation_of(activation);
     if (!(eps >= 0) || !std::isfinite(eps)) refuse("eps must be finite and >= 0, got ", eps);

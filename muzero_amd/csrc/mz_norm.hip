@@ -25,7 +25,7 @@ void choose_vector(const mz_group_norm_t* c, int* v, int* q) {
 
 int check(const mz_group_norm_t* c) {
     MZ_REQUIRE(c != nullptr, "config is NULL");
-    MZ_REQUIRE(c->batch >= 0 && c->positions >= 0 && c->channels >= 1 && c->channels <= 1 << 24, "bad sizes in mz_group_norm_t");
+    MZ_REQUIRE(c->batch >= 0 && c->positions >= 0 && c->channels >= 1 && c->channels <= MZ_GROUP_NORM_MAX_CHANNELS, "bad sizes in mz_group_norm_t");
     MZ_REQUIRE(c->groups >= 1 && c->channels % c->groups == 0, "groups (%d) must divide channels (%d)", c->groups, c->channels);
     MZ_REQUIRE(mz::dtype_size(c->dtype), "dtype %d is not one of mz_dtype", c->dtype);
     MZ_REQUIRE(c->param_dtype == MZ_F32 || c->param_dtype == c->dtype, "param_dtype must be MZ_F32 or dtype");

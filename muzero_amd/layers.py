@@ -11,7 +11,7 @@ from .exceptions import MuZeroError
 def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, activation: Optional[str] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """activation(normalised(x) * weight + bias + residual) of channels-last states x [B, ..., C] (float32, float16,
-    bfloat16): every sample's C channels are normalised in `num_groups` groups of adjacent ones, over all positions, to
+    bfloat16; at most 2^24 channels): every sample's C channels are normalised in `num_groups` groups of adjacent ones, over all positions, to
     mean 0 and (population) variance 1.
 
     weight, bias: [C], float32 or of x's type (both alike), or None.  activation: None, 'relu', 'silu', 'gelu' (by erf) or

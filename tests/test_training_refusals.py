@@ -88,3 +88,11 @@ def test_recorded_calls_on_the_device():
             with pytest.raises(MuZeroError, match='cannot be recorded'):
                 record()
         assert torch.isfinite(call(x.clone(), z)).all()                    # and not refused any longer
+
+
+@pytest.mark.parametrize('channels', [2 ** 24 + 1, 2 ** 32 + 8, 2 ** 40])
+def test_more_channels_than_the_kernels_count(channels):
+    from muzero_amd.layers import group_norm
+    for groups in (1, channels // 8 if channels % 8 == 0 else channels):
+        with pytest.raises(MuZeroError, match='at most 16777216 channels'):
+            group_norm(torch.zeros(1, 1, 1).expand(2, 3, channels), groups)
