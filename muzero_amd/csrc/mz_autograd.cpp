@@ -76,6 +76,9 @@ void require_readable(const char* name, const OptTensor& t) {
     if (t) require_readable(name, *t);
 }
 
+// t with torch's lazy sign carried out, which t's memory does not hold
+Tensor with_sign(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // A recording of torch's operations would hold the outputs' allocation and not the kernel that fills them.
 void refuse_while_recording() {
     using c10::impl::TorchDispatchModeKey;
@@ -212,7 +215,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         mz_group_norm_t config;
         memcpy(&config, ctx->saved_data["config"].toStringRef().data(), sizeof(config));
         require_readable("the gradient", dys[0]);
-        const Tensor dy = states(dys[0], config.dy_strides);
+        const Tensor dy = states(with_sign(dys[0]), config.dy_strides);
         const auto like = [&](int input, const Tensor& t) {
             return ctx->needs_input_grad(input) ? at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)) : Tensor();
         };
@@ -286,10 +289,10 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, cons
         refuse_nodes_outside_capture(x.device(), {&x, weight ? &*weight : &x, bias ? &*bias : &x, residual ? &*residual : &x});
     {
         const at::NoGradGuard off;
-        c.x = states(x, c.config.x_strides);
-        if (residual) c.residual = states(*residual, c.config.residual_strides);
-        if (weight) c.weight = weight->contiguous();
-        if (bias) c.bias = bias->contiguous();
+        c.x = states(with_sign(x), c.config.x_strides);
+        if (residual) c.residual = states(with_sign(*residual), c.config.residual_strides);
+        if (weight) c.weight = with_sign(*weight).contiguous();
+        if (bias) c.bias = with_sign(*bias).contiguous();
         if (!differentiable) return norm_forward(c, nullptr);
     }
     return GroupNorm::apply(x, weight, bias, residual, &c);
@@ -364,28 +367,28 @@ LossCall describe(const Tensor& logits, const Tensor& targets, const OptTensor& 
     }
     require_hip(device);
     const at::NoGradGuard off;
-    c.logits = logits;
+    c.logits = with_sign(logits);
     if (rows.size() == 2) {
-        if (logits.stride(2) != 1 && classes > 1) c.logits = logits.contiguous();
+        if (c.logits.stride(2) != 1 && classes > 1) c.logits = c.logits.contiguous();
         c.config.unroll = rows[0];
         c.config.batch = rows[1];
         c.config.logits_strides[0] = c.logits.stride(0);
         c.config.logits_strides[1] = c.logits.stride(1);
     } else {
-        c.logits = logits.contiguous();
+        c.logits = c.logits.contiguous();
         c.config.unroll = 1;
         c.config.batch = c10::multiply_integers(rows);
         c.config.logits_strides[1] = classes;
     }
     if (game) {
-        c.game = game->contiguous();
-        c.position = position->contiguous();
+        c.game = with_sign(*game).contiguous();
+        c.position = with_sign(*position).contiguous();
     } else {
         c.config.target_positions = c.config.unroll;
         c.config.target_games = c.config.batch;
     }
-    if (w.defined()) c.weights = rows_of(w, c.config.weight_strides);
-    c.targets = targets.contiguous();
+    if (w.defined()) c.weights = rows_of(with_sign(w), c.config.weight_strides);
+    c.targets = with_sign(targets).contiguous();
     return c;
 }
 
@@ -393,7 +396,7 @@ std::pair<Tensor, Tensor> loss_run(LossCall& c, bool with_loss, bool with_grad, 
     Tensor loss, grad, up;
     if (with_loss) loss = at::empty(c.logits.sizes().slice(0, c.logits.dim() - 1), c.logits.options().dtype(at::kFloat));
     if (with_grad) grad = at::empty(c.logits.sizes(), c.logits.options().memory_format(at::MemoryFormat::Contiguous));
-    if (dloss.defined()) up = rows_of(dloss, c.config.dloss_strides);
+    if (dloss.defined()) up = rows_of(with_sign(dloss), c.config.dloss_strides);
     const On on(c.logits.device());
     done(mz_categorical_loss(on.stream, &c.config, data(c.logits), static_cast<const float*>(data(c.targets)), data(c.game), data(c.position),
                              static_cast<const float*>(data(c.weights)), static_cast<const float*>(data(up)),
@@ -469,6 +472,7 @@ struct TensorList {
             const Tensor& t = tensors[i];
             if (const char* why = unreadable(t)) refuse("tensor ", i, " ", why);
             if (dtype_of(t) < 0) refuse("tensor ", i, ": expected float32, float16 or bfloat16, got ", t.scalar_type());
+            if (t.is_neg()) refuse("tensor ", i, " is the lazy negative of its memory");
             if (t.device() != device) refuse("tensor ", i, " is on ", t.device(), ", expected ", device);
             if (!dense(t)) refuse("tensor ", i, " is not dense: shape ", t.sizes(), ", strides ", t.strides());
             described.push_back({t.data_ptr(), t.numel(), dtype_of(t), 0});
@@ -479,6 +483,7 @@ struct TensorList {
             for (size_t i = 0; i < n; ++i) {
                 const Tensor &t = tensors[i], &u = out[i];
                 if (const char* why = unreadable(u)) refuse("output ", i, " ", why);
+                if (u.is_neg()) refuse("output ", i, " is the lazy negative of its memory");
                 if (u.scalar_type() != t.scalar_type() || u.device() != device || u.sizes() != t.sizes() ||
                     !((u.is_contiguous() && t.is_contiguous()) || u.strides() == t.strides()))
                     refuse("output ", i, " must be like its tensor: ", t.scalar_type(), " ", t.sizes(), ", strides ", t.strides(), ", on ", device);

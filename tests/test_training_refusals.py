@@ -96,3 +96,45 @@ def test_more_channels_than_the_kernels_count(channels):
     for groups in (1, channels // 8 if channels % 8 == 0 else channels):
         with pytest.raises(MuZeroError, match='at most 16777216 channels'):
             group_norm(torch.zeros(1, 1, 1).expand(2, 3, channels), groups)
+
+
+def negatives(t):
+    """Tensors of t's values whose memory holds them negated: as a view of nothing else, and as a conjugate's imaginary part."""
+    return [torch._neg_view(-t)] + ([torch.complex(t, -t).conj().imag] if t.dtype == torch.float32 else [])
+
+
+def test_lazy_negatives_in_lists():
+    from muzero_amd.training import GradientSet, clip_by_global_norm, global_norm
+    a = torch.ones(5)
+    for n in negatives(a):
+        assert n.is_neg() and torch.equal(n, a)
+        for call in (lambda: GradientSet([a, n]), lambda: global_norm([n]), lambda: clip_by_global_norm([n], 1.0)):
+            with pytest.raises(MuZeroError, match='negative'):
+                call()
+    with pytest.raises(MuZeroError, match='negative'):
+        clip_by_global_norm([a], 1.0, [torch._neg_view(a.clone())])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+def test_lazy_negatives_are_read_with_their_sign(dtype):
+    from muzero_amd.layers import group_norm
+    from muzero_amd.training import categorical_loss, categorical_loss_and_grad
+    gen = torch.Generator(device='cuda').manual_seed(2)
+    noise = lambda *s: torch.randn(*s, generator=gen, device='cuda')
+    x, res, dy, w, b = noise(3, 4, 8).to(dtype), noise(3, 4, 8).to(dtype), noise(3, 4, 8).to(dtype), noise(8).to(dtype), noise(8).to(dtype)
+    z, t, weights, up = noise(2, 3, 5).to(dtype), noise(2, 3, 5).abs(), noise(2, 3).abs(), noise(2, 3)
+
+    def run(x, w, b, res, dy, z, t, weights, up):
+        leaves = [v.detach().requires_grad_() for v in (x, w, b, res, z)]
+        y = group_norm(leaves[0], 2, leaves[1], leaves[2], activation='silu', residual=leaves[3])
+        loss = categorical_loss(leaves[4], t, weights=weights)
+        return [y, loss, *torch.autograd.grad(y, leaves[:4], dy), *torch.autograd.grad(loss, leaves[4], up), group_norm(x, 2, w, b, residual=res),
+                *categorical_loss_and_grad(z, t, weights=weights)]
+
+    args = [x, w, b, res, dy, z, t, weights, up]
+    want = run(*args)
+    for i, arg in enumerate(args):
+        for n in negatives(arg):
+            assert n.is_neg()
+            assert all(torch.equal(p, q) for p, q in zip(run(*args[:i], n, *args[i + 1:]), want)), i
