@@ -456,6 +456,11 @@ bool dense(const Tensor& t) {
     return true;
 }
 
+// one element's place in both is the same
+bool alike(const Tensor& t, const Tensor& u) {
+    return t.sizes() == u.sizes() && ((t.is_contiguous() && u.is_contiguous()) || t.strides() == u.strides());
+}
+
 struct TensorList {
     std::vector<Tensor> tensors, out;
     std::vector<mz_tensor_t> described;
@@ -484,18 +489,23 @@ struct TensorList {
                 const Tensor &t = tensors[i], &u = out[i];
                 if (const char* why = unreadable(u)) refuse("output ", i, " ", why);
                 if (u.is_neg()) refuse("output ", i, " is the lazy negative of its memory");
-                if (u.scalar_type() != t.scalar_type() || u.device() != device || u.sizes() != t.sizes() ||
-                    !((u.is_contiguous() && t.is_contiguous()) || u.strides() == t.strides()))
+                if (u.scalar_type() != t.scalar_type() || u.device() != device || !alike(u, t))
                     refuse("output ", i, " must be like its tensor: ", t.scalar_type(), " ", t.sizes(), ", strides ", t.strides(), ", on ", device);
                 outputs.push_back(u.data_ptr());
             }
         }
         require_hip(device);
     }
-    void check_unmoved() const {
-        for (size_t i = 0; i < tensors.size(); ++i)
-            if (tensors[i].data_ptr() != described[i].data || (!outputs.empty() && out[i].data_ptr() != outputs[i]))
-                refuse("tensor ", i, " or its output has other memory than when the set was made");
+    // every tensor is where it was, of the size and type it had, and dense
+    void check_unchanged() const {
+        const auto same = [&](const Tensor& t, const mz_tensor_t& was, void* data) {
+            return t.data_ptr() == data && t.numel() == was.elements && dtype_of(t) == was.dtype && dense(t);
+        };
+        for (size_t i = 0; i < tensors.size(); ++i) {
+            if (!same(tensors[i], described[i], described[i].data) || (!outputs.empty() && !same(out[i], described[i], outputs[i])))
+                refuse("tensor ", i, " or its output has other memory, or another shape or type, than when the set was made");
+            if (!outputs.empty() && !alike(out[i], tensors[i])) refuse("tensor ", i, " and its output are laid out unlike each other");
+        }
     }
     const std::vector<Tensor>& written() const { return outputs.empty() ? tensors : out; }
     void* const* output_table() const { return outputs.empty() ? nullptr : outputs.data(); }
@@ -562,7 +572,7 @@ class GradientSet {
         memory_ = host.to(list_.device);
     }
     Tensor global_norm() const {
-        list_.check_unmoved();
+        list_.check_unchanged();
         void* const table = this->table();
         return list_.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
             return mz_tensor_table_global_norm(stream, &table_, table, ws, bytes, norm);
@@ -571,7 +581,7 @@ class GradientSet {
     Tensor clip_by_global_norm(double max_norm) const {
         list_.check_clip(max_norm);
         if (!overlap_.empty()) refuse("cannot clip: ", overlap_);
-        list_.check_unmoved();
+        list_.check_unchanged();
         void* const table = this->table();
         const Tensor norm = list_.run([&](void* stream, void* ws, int64_t bytes, float* norm) {
             return mz_tensor_table_clip(stream, &table_, table, max_norm, ws, bytes, norm);

@@ -504,3 +504,31 @@ def test_second_derivatives_of_the_loss_are_refused():
     (g,) = torch.autograd.grad(categorical_loss(z, block(4, 1, 9)[:, 0]).sum(), z, create_graph=True)
     with pytest.raises(RuntimeError, match='differentiable once'):
         g.sum().backward()
+
+
+@pytest.mark.parametrize('change', [lambda t: t.resize_(4), lambda t: t.set_(t.view(torch.int32)[:4].view(F32)), lambda t: t.as_strided_((4, 2), (4, 1))],
+                         ids=['resized', 'shorter', 'strided'])
+@pytest.mark.parametrize('which', ['tensor', 'output'])
+def test_a_set_whose_tensor_was_given_another_shape_is_refused(which, change):
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.training import GradientSet
+    memory = torch.ones(64, device='cuda')
+    a, b, c, d = (memory[i:i + 8] for i in (0, 8, 24, 32))
+    kept = GradientSet([a, b], [c, d])
+    kept.clip_by_global_norm(1.0)
+    before = memory.clone()
+    change(b if which == 'tensor' else d)
+    for call in (kept.global_norm, lambda: kept.clip_by_global_norm(1.0)):
+        with pytest.raises(MuZeroError, match='than when the set was made|unlike each other'):
+            call()
+    assert torch.equal(memory, before)
+
+
+def test_a_set_whose_tensor_was_viewed_in_another_order_is_refused():
+    from muzero_amd.exceptions import MuZeroError
+    from muzero_amd.training import GradientSet
+    a, out = torch.randn(3, 4, device='cuda'), torch.empty(3, 4, device='cuda')
+    kept = GradientSet([a], [out])
+    a.as_strided_((3, 4), (1, 3))                                         # dense, of the same size, at the same address
+    with pytest.raises(MuZeroError, match='unlike each other'):
+        kept.clip_by_global_norm(1.0)
