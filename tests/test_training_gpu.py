@@ -532,3 +532,17 @@ def test_a_set_whose_tensor_was_viewed_in_another_order_is_refused():
     a.as_strided_((3, 4), (1, 3))                                         # dense, of the same size, at the same address
     with pytest.raises(MuZeroError, match='unlike each other'):
         kept.clip_by_global_norm(1.0)
+
+
+def test_more_rows_of_a_step_than_one_grid_holds():
+    """2^26 rows and more at 64 lanes a row: 2^32 threads side by side."""
+    from muzero_amd.training import categorical_loss
+    B, C, G = 2 ** 26 + 5, 300, 3
+    targets, z = block(1, G, C, 7, zero=0), torch.randn(C, device='cuda').half()
+    game = torch.arange(B, device='cuda', dtype=torch.int32) % G
+    game[-3:] = torch.tensor([2, 2, G], dtype=torch.int32)               # the last one outside
+    position = torch.zeros(1, dtype=torch.int32, device='cuda').expand(B)
+    few = categorical_loss(z.expand(1, G, C), targets, torch.arange(G, device='cuda'), torch.zeros(G, dtype=torch.int64, device='cuda'))
+    check('loss', few, to.categorical(f64(z.expand(G, C)), f64(targets[0]))[0], to.categorical_bounds(f64(z.expand(G, C)), f64(targets[0]))[0], F32)
+    loss = categorical_loss(z.expand(1, B, C), targets, game, position)[0]
+    assert torch.isnan(loss[-1]) and torch.equal(loss[:-1], few[0][game[:-1].long()])
