@@ -761,11 +761,11 @@ __global__ void __launch_bounds__(kSplitThreads) norm_back_apply_kernel(Norm d) 
 // ---- dweight, dbias ---------------------------------------------------------------------------------------------------
 
 // ws [rows][2][C] summed over its rows: 8 columns a workgroup, 128 rows side by side, in 64 bits (sums over every position
-// of a batch, which may cancel)
+// of a batch, which may cancel).  `first`: a launch's first column
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_params_kernel(Norm d, long rows) {
+__global__ void __launch_bounds__(1024) norm_params_kernel(Norm d, long rows, int first) {
     __shared__ double part[16][8];
-    const int t = threadIdx.x, c = blockIdx.x * 8 + (t & 7), column = c < 2 * d.C ? c : 2 * d.C - 1;
+    const int t = threadIdx.x, c = first + blockIdx.x * 8 + (t & 7), column = c < 2 * d.C ? c : 2 * d.C - 1;
     double s = 0.0;
     for (long r = t >> 3; r < rows; r += 8 * 128) {
         float v[8];
@@ -853,8 +853,9 @@ void backward(const Plan& p, hipStream_t st) {
                 if (d.dx || d.dres) norm_back_apply_kernel<T, V, Q><<<grid, kSplitThreads, 0, st>>>(d);
             }
         });
-    if (d.dw || d.db)           // of no rows: zeros
-        norm_params_kernel<T><<<(2 * d.C + 7) / 8, 1024, 0, st>>>(d, empty ? 0 : p.k ? d.blocks : d.N * d.splits);
+    const int most = 1 << 23;   // columns of a launch: a grid holds fewer than 2^32 threads side by side
+    for (int c = 0; (d.dw || d.db) && c < 2 * d.C; c += most)          // of no rows: zeros
+        norm_params_kernel<T><<<((2 * d.C - c < most ? 2 * d.C - c : most) + 7) / 8, 1024, 0, st>>>(d, empty ? 0 : p.k ? d.blocks : d.N * d.splits, c);
 }
 
 extern template void forward<float>(const Plan&, hipStream_t);

@@ -97,3 +97,10 @@ def test_samples_and_positions_far_apart(case, which):
     if which in ('dy', 'all'):
         dy = spread(dy, batch_stride, position_stride)
     run_and_check(x, G, w, b, activation, res, dy)
+
+
+# 2^25 sums of dweight and dbias: eight columns a workgroup of 1024 threads are 2^32 threads, more than one grid holds
+@pytest.mark.parametrize('case', [(1, (), 2 ** 24, 2 ** 21, F16, None, False, 'f32'), (2, (), 2 ** 23 + 4, 1, F32, None, False, 'f32'),
+                                  (1, (), 2 ** 24, 2 ** 24, BF16, None, True, 'same')], ids=name_of)
+def test_as_many_channels_as_there_may_be(case):
+    run_and_check(*make(case, 3))
