@@ -124,16 +124,24 @@ __global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double* par
     if (threadIdx.x == 0) *out_norm = (float)norm;
 }
 
-template <typename T>
-__device__ inline void scale_chunk(const T* in, T* out, long n, float f) {
+// F: float, or double for a scale below float's smallest normal number, which would lose bits that the product has
+template <typename T, typename F>
+__device__ inline void scale_chunk(const T* in, T* out, long n, F f) {
     walk<false>(in, n,
          [&](long i, const Vec<T, 16 / sizeof(T)>& v) {
              float r[16 / sizeof(T)];
 #pragma unroll
-             for (int k = 0; k < (int)(16 / sizeof(T)); ++k) r[k] = v[k] * f;
+             for (int k = 0; k < (int)(16 / sizeof(T)); ++k) r[k] = (float)(v[k] * f);
              mz::store(out + i, r);
          },
-         [&](long i) { out[i] = (T)((float)in[i] * f); });
+         [&](long i) { out[i] = (T)(float)((float)in[i] * f); });
+}
+
+template <typename F>
+__device__ inline void scale_part(const Entry& e, long at, long n, F f) {
+    if (e.dtype == MZ_F32) scale_chunk(static_cast<const float*>(e.in) + at, static_cast<float*>(e.out) + at, n, f);
+    else if (e.dtype == MZ_F16) scale_chunk(static_cast<const f16*>(e.in) + at, static_cast<f16*>(e.out) + at, n, f);
+    else scale_chunk(static_cast<const bf16*>(e.in) + at, static_cast<bf16*>(e.out) + at, n, f);
 }
 
 template <typename Table>
@@ -142,14 +150,14 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(Table t, const double* p
     const Entry* e = t.entries();
     const double norm = norm_of(partials, n, scratch);
     if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) *out_norm = (float)norm;
-    const float f = norm <= max_norm ? 1.f : (float)(max_norm / norm);        // a NaN norm gives NaN
+    const double scale = norm <= max_norm ? 1.0 : max_norm / norm;            // a NaN norm gives NaN
+    const float f = (float)scale;
     for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
         const int i = tensor_of(e, t.n, chunk);
         if (f == 1.f && e[i].in == e[i].out) continue;                        // nothing to change in place
         const long at = (chunk - e[i].first) * t.chunk, m = e[i].elements - at < t.chunk ? e[i].elements - at : t.chunk;
-        if (e[i].dtype == MZ_F32) scale_chunk(static_cast<const float*>(e[i].in) + at, static_cast<float*>(e[i].out) + at, m, f);
-        else if (e[i].dtype == MZ_F16) scale_chunk(static_cast<const f16*>(e[i].in) + at, static_cast<f16*>(e[i].out) + at, m, f);
-        else scale_chunk(static_cast<const bf16*>(e[i].in) + at, static_cast<bf16*>(e[i].out) + at, m, f);
+        if (scale > 0.0 && scale < 0x1p-126) scale_part(e[i], at, m, scale);
+        else scale_part(e[i], at, m, f);
     }
 }
 

@@ -71,8 +71,9 @@ class GradientSet:
 
     def clip_by_global_norm(self, max_norm: float) -> torch.Tensor:
         """Writes every tensor times max_norm / global norm to its output where the norm is above max_norm, else unchanged,
-        and returns the norm before clipping.  Where that is NaN every output is NaN; where it is infinite, finite elements
-        become 0 and infinite ones NaN."""
+        and returns the norm before clipping.  Where that is NaN every output is NaN; where an element is infinite, finite ones
+        become 0 and infinite ones NaN.  (A norm of finite elements above float32's range is returned as infinite, and clipped by
+        all the same.)"""
         try:
             return self._set.clip_by_global_norm(max_norm)
         except TypeError:

@@ -546,3 +546,22 @@ def test_more_rows_of_a_step_than_one_grid_holds():
     check('loss', few, to.categorical(f64(z.expand(G, C)), f64(targets[0]))[0], to.categorical_bounds(f64(z.expand(G, C)), f64(targets[0]))[0], F32)
     loss = categorical_loss(z.expand(1, B, C), targets, game, position)[0]
     assert torch.isnan(loss[-1]) and torch.equal(loss[:-1], few[0][game[:-1].long()])
+
+
+@pytest.mark.parametrize('dtypes', [(F32,), (BF16,), (F32, BF16)], ids=['f32', 'bf16', 'mixed'])
+@pytest.mark.parametrize('size,max_norm', [(1e10, 1e-29), (1e30, 1e-12), (1e5, 1e-37), (3e30, 1e-300)])
+def test_scales_below_the_smallest_normal_number(size, max_norm, dtypes):
+    """max_norm / norm as a float32 would have lost bits, or all of them, though the products are ordinary numbers."""
+    from muzero_amd.training import GradientSet, clip_by_global_norm
+    tensors = tensors_of([1000, 3, 70001], dtypes, scale=size)
+    out, kept = [torch.full_like(t, 7) for t in tensors], [t.clone() for t in tensors]
+    check_clip(tensors, max_norm, out, clip_by_global_norm(tensors, max_norm, out=out))
+    GradientSet(kept).clip_by_global_norm(max_norm)
+    assert all(torch.equal(a, b) for a, b in zip(out, kept))
+
+
+def test_norms_above_the_range_of_float32():
+    from muzero_amd.training import GradientSet
+    t = torch.full((1 << 20,), 3e38, device='cuda')
+    assert math.isinf(float(GradientSet([t]).clip_by_global_norm(1.0)))
+    assert torch.allclose(t, torch.full_like(t, 2.0 ** -10), rtol=3 * to.U32, atol=0)
