@@ -91,7 +91,6 @@ void refuse_while_recording() {
 }
 
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-void* data(const OptTensor& t) { return t ? data(*t) : nullptr; }
 bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
 
 // The device of the call made current, and its current stream
