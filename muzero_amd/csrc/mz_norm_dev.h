@@ -177,8 +177,10 @@ struct Cut {
     __device__ float operator()(float z) const { return z < floor ? floor : z; }              // a NaN stays
     __device__ float slope(float z) const { return z <= edge ? 0.f : 1.f; }
 };
-// The others from one exponential and one reciprocal, each within a step or two of f32 (v_exp_f32, v_rcp_f32): with the
-// library's exact division, erf and tanh the arithmetic took longer than the memory.
+// The others from one exponential and one reciprocal of the hardware (v_exp_f32, v_rcp_f32, one step each): with the library's
+// exact division, erf and tanh the arithmetic took longer than the memory.  The exponent is a rounded product, so exp(x) is off
+// by up to (1.3 |x| + 2) 2^-24 of itself: silu by up to (1.3 |z| + 8) 2^-24 of itself, tanh, whose exponential counts for less
+// the farther out it is, by 12 2^-24.  A reciprocal below 2^-126 is 0: silu below -87.
 __device__ inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950409f); }
 __device__ inline float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
@@ -191,9 +193,10 @@ struct Silu {
         return s * fmaf(z, 1.f - s, 1.f);
     }
 };
-// z times the normal distribution's integral, by the five-term approximation of Abramowitz and Stegun 7.1.26 (off by at most
-// 1.5e-7 / 2 everywhere, relatively good in the lower tail, where it is taken as it stands), with the exponential that the
-// density needs too.
+// z times the normal distribution's integral, by the five-term approximation of Abramowitz and Stegun 7.1.26, with the
+// exponential that the density needs too.  Off by 1.5e-7 / 2 at most and as much again or twice by f32's sums: 2.7e-7 |z|
+// measured over [-10, 10].  That is absolute, as for 1 + erf: in the lower tail it is a growing part of the value (5e-4 at -4,
+// 1.6e-3 at -5, 1e-2 at -8, where gelu is 5e-15).
 struct Gelu {
     __device__ explicit Gelu(int) {}
     __device__ static float below(float z, float e) {          // e = exp(-z^2 / 2)

@@ -337,3 +337,43 @@ def test_capture_is_refused_through_the_graph_in_front_as_well():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             group_norm(eager, 4)
     assert torch.isfinite(group_norm(eager, 4)).all()
+
+
+@pytest.mark.parametrize('activation', [None, 'relu', 'silu', 'gelu', 'tanh'])
+def test_activations_over_their_whole_range(activation):
+    """With weights of 0 the activation's argument is the residual itself, and dresidual of ones the slope.  u = 2^-24: a rounding;
+    the hardware's exponential and reciprocal 2 u, and the exponential's argument one more, which is |x| u / ln 2 of it or less:
+    (1.3 |x| + 2) u with the constant's own.
+      silu   exp, 1 + e, reciprocal, product: (1.3 |z| + 8) u; the slope s (1 + z (1 - s)) as much of each of its two terms
+      tanh   (1 - q) / (1 + q), q = exp(-2 |z|) off by q (2.6 |z| + 2) u < 2 u, 1 - q > 0.39 where it is used: 12 u with the rest;
+             the slope 4 q / (1 + q)^2 (2.6 |z| + 12) u
+      gelu   the integral: 7.5e-8 (five terms), 12 u (sums of terms that alternate and add up to 2.24); its density 4 u of itself and
+             0.65 z^2 u of 0.4 |z| exp(-z^2 / 2), both under u"""
+    from muzero_amd.layers import group_norm
+    side = torch.cat([torch.logspace(-30, 2, 40000, device='cuda'), torch.linspace(0, 12, 84768, device='cuda'), torch.linspace(12, 88, 6304, device='cuda')])
+    z = torch.cat([side, -side]).reshape(1, -1, 16)
+    w, leaf = torch.zeros(16, device='cuda'), z.clone().requires_grad_()
+    y = group_norm(torch.randn_like(z), 4, w, activation=activation, residual=leaf)
+    (slope,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    z, y, slope = f64(z).ravel(), f64(y).ravel(), f64(slope).ravel()
+    with np.errstate(over='ignore'):
+        want, want_slope = to.act(z, activation), to.act_slope(z, activation)
+    # tiny: a reciprocal below 2^-126, the smallest normal number, may be 0; times |z| <= 100
+    u, a, tiny = to.U32, np.abs(z), 100 * 2.0 ** -126
+    if activation == 'gelu':
+        from math import erfc
+        phi = np.array([0.5 * erfc(-v / 2 ** 0.5) for v in z])
+        want, want_slope = z * phi, phi + z * np.exp(-z * z / 2) / (2 * np.pi) ** 0.5
+        off, off_slope = a * (7.5e-8 + 12 * u) + u * np.abs(want) + tiny, 7.5e-8 + 12 * u + 3 * u
+    elif activation == 'silu':
+        with np.errstate(over='ignore'):
+            s = 1 / (1 + np.exp(-z))
+        off, off_slope = (1.3 * a + 8) * u * np.abs(want) + tiny, (1.3 * a + 10) * u * (s + np.abs(z * s * (1 - s))) + a * s * 8 * u + tiny
+    elif activation == 'tanh':
+        want_slope = 1 / np.cosh(z) ** 2
+        off, off_slope = 12 * u * np.abs(want) + tiny, (2.6 * a + 12) * u * want_slope + tiny
+    else:
+        off = off_slope = 0.0 * a
+    for got, exact, bound in ((y, want, off), (slope, want_slope, off_slope)):
+        far = np.abs(got - exact) - bound
+        assert (far <= 0).all(), f'{got[far.argmax()]:.9g} at {z[far.argmax()]:.9g}, expected {exact[far.argmax()]:.9g}'
