@@ -3,7 +3,8 @@ global gradient norm and clipping by it (csrc/mz_clip.hip).  The reference leave
 the names follow its framework.
 
 A forward pass that is being captured into a graph is refused where its backward pass would reach an autograd node of a stream
-outside the capture (an eager graph of the same leaves that is still alive)."""
+outside the capture (an eager graph of the same leaves that is still alive).  Forward-mode derivatives, transforms of torch.func
+and recordings of torch's operations (torch.jit.trace, torch.fx, torch.export, fake tensors) are refused."""
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -54,12 +55,14 @@ def _list(fn, tensors, *args):
 class GradientSet:
     """The gradients of a network whose buffers stay where they are from step to step (zeroed in place, or written by a
     captured graph): their table is checked once and kept on the device, and `global_norm()` and
-    `clip_by_global_norm(max_norm)` cost two launches each, whatever the number of tensors.
+    `clip_by_global_norm(max_norm)` cost two launches each, whatever the number of tensors.  With torch's optimisers that is
+    optimizer.zero_grad(set_to_none=False): by default every backward pass makes new .grad tensors, of which the set knows
+    nothing; clip_by_global_norm() below takes those.
 
     tensors: 1 to 8192 float32, float16 and bfloat16 tensors of one device, each dense in some order of its dimensions.
     out: the tensors that clipping writes, of the same shapes, strides and types; None = the tensors themselves.  The set
     keeps the tensors alive, and has to be kept as long as a graph with calls of it is replayed; it is made outside
-    captures.  A tensor that was given other memory since is refused.  Results are ordered on the current stream; a set may be
+    captures.  A tensor that was given other memory or another shape since is refused.  Results are ordered on the current stream; a set may be
     used on several streams at once."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None) -> None:
@@ -82,7 +85,7 @@ class GradientSet:
 
 def global_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     """GradientSet(tensors).global_norm() for tensors that are others in every step: their table travels with the launch, 112
-    tensors each, and nothing is uploaded."""
+    tensors each, and nothing is uploaded.  Outside autograd: the norm has no gradient."""
     return _list(_lib.native().global_norm, tensors)
 
 

@@ -565,3 +565,30 @@ def test_norms_above_the_range_of_float32():
     t = torch.full((1 << 20,), 3e38, device='cuda')
     assert math.isinf(float(GradientSet([t]).clip_by_global_norm(1.0)))
     assert torch.allclose(t, torch.full_like(t, 2.0 ** -10), rtol=3 * to.U32, atol=0)
+
+
+@pytest.mark.parametrize('keep', [True, False], ids=['kept', 'new'])
+def test_clipping_between_a_backward_pass_and_the_optimiser(keep):
+    """Both ways of the usual loop: .grad tensors zeroed in place and a set made once, or new ones in every step."""
+    from muzero_amd.layers import group_norm
+    from muzero_amd.training import GradientSet, categorical_loss, clip_by_global_norm
+    gen = torch.Generator(device='cuda').manual_seed(6)
+    x, t = torch.randn(33, 9, 16, generator=gen, device='cuda'), block(33, 1, 7, 2, zero=0)[:, 0]
+    params = [torch.randn(16, generator=gen, device='cuda').requires_grad_(), torch.zeros(16, device='cuda', requires_grad=True),
+              torch.randn(144, 7, generator=gen, device='cuda').requires_grad_()]
+    optimiser, gradients = torch.optim.SGD(params, lr=0.5), None
+    for step in range(3):
+        optimiser.zero_grad(set_to_none=not keep)
+        h = group_norm(x, 4, params[0], params[1], activation='silu')
+        categorical_loss(h.reshape(33, -1) @ params[2], t).sum().backward()
+        before, was = [p.grad.clone() for p in params], [p.detach().clone() for p in params]
+        if keep:
+            gradients = gradients or GradientSet([p.grad for p in params])
+            norm = gradients.clip_by_global_norm(0.01)
+        else:
+            norm = clip_by_global_norm([p.grad for p in params], 0.01)
+        assert float(norm) > 0.01
+        check_clip(before, 0.01, [p.grad for p in params], norm)
+        optimiser.step()
+        for p, w in zip(params, was):
+            assert torch.allclose(p, w - 0.5 * p.grad, rtol=4 * to.U32, atol=1e-30)
