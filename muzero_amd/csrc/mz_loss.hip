@@ -27,8 +27,9 @@ constexpr int kMaxClasses = 4096;
 constexpr float kLog2e = 1.4426950409f;
 
 struct Loss {
-    long U, B, P, G, u0, b0;            // u0, b0: first step and row of a launch
+    long U, B, P, G, u0;                // u0: first step of a launch
     int C, wide, lanes, last;           // wide: 8-byte indexes; lanes of a row, a lane's last chunk
+    uint32_t block0;                    // workgroups of a step that earlier launches had
     long zs[2], ws[2], gs[2];
     const void* z;
     const float *t, *w, *g;
@@ -45,7 +46,7 @@ __device__ inline long index_at(const void* p, int wide, long i) {
 template <typename T, int V, int K, bool LOSS, bool GRAD>
 __global__ void __launch_bounds__(kThreads) categorical_kernel(Loss d) {
     const int lane = threadIdx.x & (d.lanes - 1), last = K <= 4 ? K - 1 : d.last;
-    const long u = d.u0 + blockIdx.y, b = d.b0 + blockIdx.x * (long)(kThreads / d.lanes) + threadIdx.x / d.lanes;
+    const long u = d.u0 + blockIdx.y, b = (d.block0 + blockIdx.x) * (long)(kThreads / d.lanes) + threadIdx.x / d.lanes;
     if (b >= d.B) return;                                    // all lanes of a row
     // The lane's chunk k.  One that would pass the row's end is moved back to end with it: of the last chunk, the first `twice`
     // classes belong to another lane (all V or more: the lane has no such chunk) and neither count nor are stored.
@@ -149,11 +150,12 @@ void launch(Loss d, hipStream_t st) {
     d.last = k - 1;
     const long rows = kThreads / d.lanes;
     // what a grid may hold: fewer than 2^32 threads side by side, and 65535 steps
-    const long most_rows = rows << 23, most_steps = 65535;
+    const long blocks = (d.B + rows - 1) / rows, most_blocks = 1 << 23, most_steps = 65535;
     for (; d.u0 < d.U; d.u0 += most_steps)
-        for (d.b0 = 0; d.b0 < d.B; d.b0 += most_rows) {
-            const long b = d.B - d.b0 < most_rows ? d.B - d.b0 : most_rows, u = d.U - d.u0 < most_steps ? d.U - d.u0 : most_steps;
-            const dim3 grid((unsigned)((b + rows - 1) / rows), (unsigned)u);
+        for (long first = 0; first < blocks; first += most_blocks) {
+            d.block0 = (uint32_t)first;
+            const dim3 grid((unsigned)(blocks - first < most_blocks ? blocks - first : most_blocks),
+                            (unsigned)(d.U - d.u0 < most_steps ? d.U - d.u0 : most_steps));
             if (v == 1) k == 1 ? launch<T, 1, 1>(d, grid, st) : launch<T, 1, 2>(d, grid, st);
             else if (k == 1) launch<T, 4, 1>(d, grid, st);
             else if (k == 2) launch<T, 4, 2>(d, grid, st);
