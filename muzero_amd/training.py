@@ -31,7 +31,8 @@ def categorical_loss(logits: torch.Tensor, targets: torch.Tensor, game: Optional
     row (u, b) meets targets[position[b] + u, game[b]]: no gathered copy.  An index outside the block gives NaN (the host
     does not look at them).  weights broadcast over the rows; rows of weight 0 give 0 whatever they hold.  A
     class with target 0 adds nothing, also where its logit is -inf (an illegal move); a row whose logits are all -inf gives 0.
-    A row of zero targets (past the end of a game) gives 0.  Differentiable once with respect to logits alone."""
+    A row of zero targets (past the end of a game) gives 0, unless its logits are NaN or +inf.  Differentiable once, in reverse
+    mode, with respect to logits alone."""
     return _loss(_lib.native().categorical_loss, logits, targets, game, position, weights)
 
 
