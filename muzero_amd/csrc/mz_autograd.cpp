@@ -64,7 +64,9 @@ void require_hip(const c10::Device& d) {
 // lost without a word.
 const char* unreadable(const Tensor& t) {
     if (t.layout() != at::kStrided) return "is not a strided tensor";
-    if (!t.has_storage()) return "has no memory of its own (a tensor inside a transform of torch.func, for instance)";
+    // a null pointer would pass for an input that is not given
+    if (!t.has_storage() || (t.numel() && !t._is_zerotensor() && !t.const_data_ptr()))
+        return "has no memory of its own (a tensor inside a transform of torch.func, or one that wraps others)";
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
         return "carries a forward-mode derivative: muzero_amd's training operators are differentiable in reverse mode alone";
     return nullptr;
@@ -76,8 +78,8 @@ void require_readable(const char* name, const OptTensor& t) {
     if (t) require_readable(name, *t);
 }
 
-// t with torch's lazy sign carried out, which t's memory does not hold
-Tensor with_sign(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+// t with what torch does lazily carried out, which t's memory does not hold: its sign, and zeros without any
+Tensor written_out(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t._is_zerotensor() ? t.clone() : t; }
 
 // A recording of torch's operations would hold the outputs' allocation and not the kernel that fills them.
 void refuse_while_recording() {
@@ -214,7 +216,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         mz_group_norm_t config;
         memcpy(&config, ctx->saved_data["config"].toStringRef().data(), sizeof(config));
         require_readable("the gradient", dys[0]);
-        const Tensor dy = states(with_sign(dys[0]), config.dy_strides);
+        const Tensor dy = states(written_out(dys[0]), config.dy_strides);
         const auto like = [&](int input, const Tensor& t) {
             return ctx->needs_input_grad(input) ? at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)) : Tensor();
         };
@@ -288,10 +290,10 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, cons
         refuse_nodes_outside_capture(x.device(), {&x, weight ? &*weight : &x, bias ? &*bias : &x, residual ? &*residual : &x});
     {
         const at::NoGradGuard off;
-        c.x = states(with_sign(x), c.config.x_strides);
-        if (residual) c.residual = states(with_sign(*residual), c.config.residual_strides);
-        if (weight) c.weight = with_sign(*weight).contiguous();
-        if (bias) c.bias = with_sign(*bias).contiguous();
+        c.x = states(written_out(x), c.config.x_strides);
+        if (residual) c.residual = states(written_out(*residual), c.config.residual_strides);
+        if (weight) c.weight = written_out(*weight).contiguous();
+        if (bias) c.bias = written_out(*bias).contiguous();
         if (!differentiable) return norm_forward(c, nullptr);
     }
     return GroupNorm::apply(x, weight, bias, residual, &c);
@@ -366,7 +368,7 @@ LossCall describe(const Tensor& logits, const Tensor& targets, const OptTensor& 
     }
     require_hip(device);
     const at::NoGradGuard off;
-    c.logits = with_sign(logits);
+    c.logits = written_out(logits);
     if (rows.size() == 2) {
         if (c.logits.stride(2) != 1 && classes > 1) c.logits = c.logits.contiguous();
         c.config.unroll = rows[0];
@@ -380,14 +382,14 @@ LossCall describe(const Tensor& logits, const Tensor& targets, const OptTensor& 
         c.config.logits_strides[1] = classes;
     }
     if (game) {
-        c.game = with_sign(*game).contiguous();
-        c.position = with_sign(*position).contiguous();
+        c.game = written_out(*game).contiguous();
+        c.position = written_out(*position).contiguous();
     } else {
         c.config.target_positions = c.config.unroll;
         c.config.target_games = c.config.batch;
     }
-    if (w.defined()) c.weights = rows_of(with_sign(w), c.config.weight_strides);
-    c.targets = with_sign(targets).contiguous();
+    if (w.defined()) c.weights = rows_of(written_out(w), c.config.weight_strides);
+    c.targets = written_out(targets).contiguous();
     return c;
 }
 
@@ -395,7 +397,7 @@ std::pair<Tensor, Tensor> loss_run(LossCall& c, bool with_loss, bool with_grad, 
     Tensor loss, grad, up;
     if (with_loss) loss = at::empty(c.logits.sizes().slice(0, c.logits.dim() - 1), c.logits.options().dtype(at::kFloat));
     if (with_grad) grad = at::empty(c.logits.sizes(), c.logits.options().memory_format(at::MemoryFormat::Contiguous));
-    if (dloss.defined()) up = rows_of(with_sign(dloss), c.config.dloss_strides);
+    if (dloss.defined()) up = rows_of(written_out(dloss), c.config.dloss_strides);
     const On on(c.logits.device());
     done(mz_categorical_loss(on.stream, &c.config, data(c.logits), static_cast<const float*>(data(c.targets)), data(c.game), data(c.position),
                              static_cast<const float*>(data(c.weights)), static_cast<const float*>(data(up)),
@@ -476,7 +478,7 @@ struct TensorList {
             const Tensor& t = tensors[i];
             if (const char* why = unreadable(t)) refuse("tensor ", i, " ", why);
             if (dtype_of(t) < 0) refuse("tensor ", i, ": expected float32, float16 or bfloat16, got ", t.scalar_type());
-            if (t.is_neg()) refuse("tensor ", i, " is the lazy negative of its memory");
+            if (t.is_neg() || t._is_zerotensor()) refuse("tensor ", i, " is the lazy negative of its memory, or zeros without any");
             if (t.device() != device) refuse("tensor ", i, " is on ", t.device(), ", expected ", device);
             if (!dense(t)) refuse("tensor ", i, " is not dense: shape ", t.sizes(), ", strides ", t.strides());
             described.push_back({t.data_ptr(), t.numel(), dtype_of(t), 0});
@@ -487,7 +489,7 @@ struct TensorList {
             for (size_t i = 0; i < n; ++i) {
                 const Tensor &t = tensors[i], &u = out[i];
                 if (const char* why = unreadable(u)) refuse("output ", i, " ", why);
-                if (u.is_neg()) refuse("output ", i, " is the lazy negative of its memory");
+                if (u.is_neg() || u._is_zerotensor()) refuse("output ", i, " is the lazy negative of its memory, or zeros without any");
                 if (u.scalar_type() != t.scalar_type() || u.device() != device || !alike(u, t))
                     refuse("output ", i, " must be like its tensor: ", t.scalar_type(), " ", t.sizes(), ", strides ", t.strides(), ", on ", device);
                 outputs.push_back(u.data_ptr());

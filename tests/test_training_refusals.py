@@ -138,3 +138,49 @@ def test_lazy_negatives_are_read_with_their_sign(dtype):
         for n in negatives(arg):
             assert n.is_neg()
             assert all(torch.equal(p, q) for p, q in zip(run(*args[:i], n, *args[i + 1:]), want)), i
+
+
+class Wrapper(torch.Tensor):
+    """A tensor that stands for another one: of its shape and type, with no memory."""
+    @staticmethod
+    def __new__(cls, inner):
+        self = torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+        self.inner = inner
+        return self
+
+    @classmethod
+    def __torch_dispatch__(cls, fn, types, args=(), kwargs=None):
+        return fn(*(a.inner if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+
+
+@pytest.mark.parametrize('name', calls())
+def test_tensors_that_wrap_others(name):
+    with pytest.raises(MuZeroError, match='memory of its own'):
+        calls(Wrapper)[name]()
+
+
+def test_zeros_without_memory_in_lists():
+    from muzero_amd.training import GradientSet, clip_by_global_norm
+    a, zeros = torch.ones(5), torch._efficientzerotensor(5)
+    for call in (lambda: GradientSet([a, zeros]), lambda: clip_by_global_norm([a], 1.0, [zeros])):
+        with pytest.raises(MuZeroError, match='zeros without any'):
+            call()
+
+
+@pytest.mark.gpu
+def test_wrappers_and_zeros_without_memory_on_the_device():
+    from muzero_amd.layers import group_norm
+    from muzero_amd.training import categorical_loss
+    x, w = torch.randn(2, 3, 8, device='cuda', requires_grad=True), torch.full((8,), 2.0, device='cuda')
+    z, t = torch.randn(4, 5, device='cuda', requires_grad=True), torch.ones(4, 5, device='cuda')
+    weights, index = torch.ones(4, device='cuda'), torch.zeros(4, dtype=torch.int64, device='cuda')
+    for call in (lambda: group_norm(x, 2, Wrapper(w)), lambda: group_norm(x, 2, w, Wrapper(w)), lambda: group_norm(x, 2, residual=Wrapper(x.detach())),
+                 lambda: categorical_loss(z, t, weights=Wrapper(weights)), lambda: categorical_loss(z[None], t[None], Wrapper(index), index),
+                 lambda: categorical_loss(z[None], t[None], index, Wrapper(index))):
+        with pytest.raises(MuZeroError, match='memory of its own'):
+            call()
+    none = lambda like: torch._efficientzerotensor(like.shape, device='cuda')
+    y, loss = group_norm(x, 2, none(w), none(w), residual=none(x)), categorical_loss(z, none(t), weights=weights)
+    assert (y == 0).all() and (loss == 0).all() and (categorical_loss(z, t, weights=none(weights)) == 0).all()
+    assert (torch.autograd.grad(group_norm(x, 2), x, none(x))[0] == 0).all()
+    assert (torch.autograd.grad(categorical_loss(z, t), z, none(loss))[0] == 0).all()
